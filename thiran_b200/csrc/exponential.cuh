@@ -45,10 +45,4 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return reinterpret_cast<float2&>(r);
 }
 
-// 2^(x c + b) of both halves; the exponent is rounded once.
-__device__ __forceinline__ float2 pow2Line(float2 x, float c, float b) {
-    const float2 t = fma2(x, make_float2(c, c), make_float2(b, b));
-    return make_float2(pow2(t.x), pow2(t.y));
-}
-
 } // namespace thb

@@ -96,7 +96,7 @@ constexpr bool stagesOutput(int epilogue) { return givesSlopes(epilogue) || epil
 // for each part of the columns, its first entry there.
 struct TileRows {
     uint32_t at[kLseParts][kBM], next[kLseParts][kBM], row[kBM];
-    float minusLse[kBM], scale[kBM];  // -lse in powers of two, scale * grad_loss
+    float minusLse[kBM], scale[kBM];  // scale: scale * grad_loss
 };
 
 template <bool PAIR, int EPI>
@@ -138,7 +138,7 @@ struct Params {
     const uint32_t* ids;     // [row][entries], ascending, kNoEntry behind the last
     const float* shares;     // [row][entries], null: 1
     float* listed;           // z of each list entry, [row][entries]
-    float2* strips;          // [strip][stripLd] (log2 of the shift, sum)
+    float2* strips;          // [strip][stripLd] (maximum, sum)
     uint64_t stripLd;
     // kEpiLse with few rows: each CTA folds its tiles into one strip, and the
     // last to finish joins the strips.
@@ -467,7 +467,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                     list[i] = static_cast<uint64_t>(to[i]) * p.entries;
                     out.row[r] = to[i];
                     if constexpr (givesSlopes(EPI)) {
-                        out.minusLse[r] = live[i] ? p.rowLse[row] * -kLog2e : 0.0f;
+                        out.minusLse[r] = live[i] ? -p.rowLse[row] : 0.0f;
                         out.scale[r] = live[i] ? p.rowScale[row] : 0.0f;
                     }
                 }
@@ -521,8 +521,8 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
         uint8_t* stage = base + G::stages * G::stageBytes + (warp - 2) * 32 * kStageLd;
         (void)stage;
         uint32_t rowsBuf = 0, rowsPhase = 0;
-        float runningShift = -INFINITY, runningSum = 0.0f;
-        (void)runningShift;
+        float runningTop = -INFINITY, runningSum = 0.0f;
+        (void)runningTop;
         (void)runningSum;
         const uint32_t releaseAddress = PAIR ? pairAddress(&tmemEmpty[0], 0) : 0u;
         for (uint32_t tile = first; tile < tiles; tile += step) {
@@ -610,22 +610,18 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
 #pragma unroll
                 for (uint32_t j = 0; j < kStrip; ++j) tops[j % 4] = fmaxf(tops[j % 4], z(j));
                 const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                // The sum's shift is the scaled maximum as rounded here, in
-                // powers of two, and goes with the sum: its rounding cancels.
-                // (A strip of nothing but -inf takes any finite shift.)
-                const float c = p.scale * kLog2e;
-                const float shift = top == -INFINITY ? -INFINITY : top * c;
-                const float minusShift = top == -INFINITY ? 0.0f : -shift;
+                // (A strip of nothing but -inf takes any finite maximum.)
+                const float c = p.scale * kLog2e, minusTop = top == -INFINITY ? 0.0f : -top;
                 float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (uint32_t j = 0; j < kStrip / 2; ++j)
-                    sums[j % 2] = add2(sums[j % 2], pow2Line(make_float2(z(2 * j), z(2 * j + 1)), c, minusShift));
+                    sums[j % 2] = add2(sums[j % 2], pow2Shifted(make_float2(z(2 * j), z(2 * j + 1)), minusTop, c));
                 const float2 sum = add2(sums[0], sums[1]);
                 if (p.finished)
-                    fold(runningShift, runningSum, shift, sum.x + sum.y);
+                    fold(runningTop, runningSum, top, sum.x + sum.y, c);
                 else
                     p.strips[static_cast<uint64_t>(nb * stripsOf(tileN) + part) * p.stripLd + row] =
-                        make_float2(shift, sum.x + sum.y);
+                        make_float2(top, sum.x + sum.y);
 #pragma unroll
                 for (uint32_t q = 0; q < kStrip / 32; ++q) {
                     while (next < col0 + min((q + 1) * 32, width)) {
@@ -657,10 +653,10 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                 else release();
                 const uint32_t left = p.n > col ? p.n - col : 0u;  // columns of the chunk inside C
                 if constexpr (givesSlopes(EPI)) {
-                    const float2 slope2 = make_float2(rowScale, rowScale);
+                    const float2 slope2 = make_float2(rowScale, rowScale), scale2 = make_float2(p.scale, p.scale);
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        const float2 e = mul2(slope2, pow2Line(make_float2(v[j], v[j + 1]), p.scale * kLog2e, minusLse));
+                        const float2 e = mul2(slope2, pow2Shifted(mul2(make_float2(v[j], v[j + 1]), scale2), minusLse, kLog2e));
                         v[j] = e.x;
                         v[j + 1] = e.y;
                     }
@@ -738,7 +734,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
             }
         }
         if constexpr (EPI == kEpiLse) {
-            if (p.finished && quadrant == 0) parts[part][lane] = make_float2(runningShift, runningSum);
+            if (p.finished && quadrant == 0) parts[part][lane] = make_float2(runningTop, runningSum);
         }
     }
     __syncthreads();
@@ -749,10 +745,11 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
             // z of its list entries are stored too, by the warps above.)
             __threadfence();
             __syncthreads();
+            const float c = p.scale * kLog2e;
             if (warp == 0) {
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-                for (uint32_t k = 0; k < kParts; ++k) fold(top, sum, parts[k][lane].x, parts[k][lane].y);
+                for (uint32_t k = 0; k < kParts; ++k) fold(top, sum, parts[k][lane].x, parts[k][lane].y, c);
                 if (lane < m) p.strips[lane * step + first] = make_float2(top, sum);
                 __threadfence();
                 __syncwarp();
@@ -767,7 +764,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                     float top = -INFINITY, sum = 0.0f, target = 0.0f;
                     for (uint32_t s = lane; s < step; s += 32) {
                         const float2 x = __ldcg(p.strips + row * step + s);
-                        fold(top, sum, x.x, x.y);
+                        fold(top, sum, x.x, x.y, c);
                     }
                     for (uint32_t e = lane; e < p.entries; e += 32) {
                         if (p.ids[to * p.entries + e] == kNoEntry) break;  // the list is sorted
@@ -780,10 +777,10 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                     for (uint32_t o = 1; o < 32; o *= 2) {
                         const float otherTop = __shfl_xor_sync(0xffffffffu, top, o);
                         const float otherSum = __shfl_xor_sync(0xffffffffu, sum, o);
-                        fold(top, sum, otherTop, otherSum);
+                        fold(top, sum, otherTop, otherSum, c);
                         target += __shfl_xor_sync(0xffffffffu, target, o);
                     }
-                    if (lane == 0) closeRow(to, top, sum, target, p.entropy, p.loss, p.lse);
+                    if (lane == 0) closeRow(to, top, sum, p.scale, target, p.entropy, p.loss, p.lse);
                 }
             }
         }
@@ -1156,13 +1153,13 @@ __global__ void __launch_bounds__(kPlanThreads) planRows(const PlanParams p, uin
 // kJoinRows packed rows per CTA; 64 threads fold the strips of a row (stored
 // row-fastest: eight rows are 64 bytes) and share its list, first within a
 // warp, then over the warps in order. One thread closes the loss
-//   lse = shift log(2) + log(sum),  loss = sum q log q - sum q z + lse.
+//   lse = scale maximum + log(sum),  loss = sum q log q - sum q z + lse.
 constexpr uint32_t kJoinRows = 8, kJoinThreads = 512;
 
 __global__ void __launch_bounds__(kJoinThreads)
     joinStrips(const float2* strips, uint64_t stripLd, uint32_t stripCount, const uint32_t* count, const uint32_t* rowMap,
                const uint32_t* ids, const float* shares, const float* listed, const float* entropy, uint32_t entries,
-               float* loss, float* lse) {
+               float scale, float* loss, float* lse) {
     constexpr uint32_t kWarps = kJoinThreads / 32, kGroups = kJoinThreads / kJoinRows;
     __shared__ float tops[kWarps][kJoinRows], sums[kWarps][kJoinRows], targets[kWarps][kJoinRows];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -1171,6 +1168,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     gridDependencyWait();
     const uint32_t row = blockIdx.x * kJoinRows + mine;
     const bool live = row < *count;
+    const float c = scale * kLog2e;
     float top = -INFINITY, sum = 0.0f, target = 0.0f;
     uint64_t to = 0;
     if (live) {
@@ -1178,7 +1176,7 @@ __global__ void __launch_bounds__(kJoinThreads)
 #pragma unroll 4
         for (uint32_t s = group; s < stripCount; s += kGroups) {
             const float2 x = strips[s * stripLd + row];
-            fold(top, sum, x.x, x.y);
+            fold(top, sum, x.x, x.y, c);
         }
         for (uint32_t e = group; e < entries; e += kGroups) {
             if (ids[to * entries + e] == kNoEntry) break;  // the list is sorted
@@ -1189,7 +1187,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     }
 #pragma unroll
     for (uint32_t o = kJoinRows; o < 32; o *= 2) {
-        fold(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
+        fold(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o), c);
         target += __shfl_xor_sync(0xffffffffu, target, o);
     }
     if (lane < kJoinRows) {
@@ -1200,10 +1198,10 @@ __global__ void __launch_bounds__(kJoinThreads)
     __syncthreads();
     if (threadIdx.x < kJoinRows && live) {
         for (uint32_t w = 1; w < kWarps; ++w) {
-            fold(top, sum, tops[w][mine], sums[w][mine]);
+            fold(top, sum, tops[w][mine], sums[w][mine], c);
             target += targets[w][mine];
         }
-        closeRow(to, top, sum, target, entropy, loss, lse);
+        closeRow(to, top, sum, scale, target, entropy, loss, lse);
     }
 }
 
@@ -1751,7 +1749,7 @@ cudaError_t forward(const Problem& q, int smCount, std::uint32_t* status, cudaSt
     if (e != cudaSuccess || few) return e;
     return launch(joinStrips, static_cast<uint32_t>((q.rows + kJoinRows - 1) / kJoinRows), kJoinThreads, 0, stream, 1,
                   p.strips, p.stripLd, static_cast<uint32_t>(l.stripCount), p.count, p.rowMap, p.ids, p.shares, p.listed,
-                  q.labels ? nullptr : place<float>(q, l.entropy), p.entries, q.loss, q.lse);
+                  q.labels ? nullptr : place<float>(q, l.entropy), p.entries, q.scale, q.loss, q.lse);
 }
 
 cudaError_t backward(const Problem& q, int smCount, std::uint32_t* status, cudaStream_t stream) {

@@ -4,7 +4,7 @@
 // Up to kScoreRows rows the products are small beside the weights that they
 // read, so that the weights are streamed once through plain loads, each
 // element multiplied with the rows' elements from shared memory. A warp takes
-// a run of weight rows, four at a time, and keeps a running (shift, sum) for
+// a run of weight rows, four at a time, and keeps a running (maximum, sum) for
 // every row. No packing and no copies: rows of weights at any address are read
 // in the aligned 16-byte vectors that hold them, against H shifted as far. Rows
 // with the same shift are `classes` apart; a CTA takes those of one class.
@@ -45,7 +45,7 @@ struct ScoreParams {
     const uint32_t* ids;     // [row][entries], ascending, kNoEntry behind the last
     const float* shares;     // [row][entries]
     const float* entropy;    // [row]
-    float2* strips;          // [row][CTA] (shift in powers of two, sum)
+    float2* strips;          // [row][CTA] (maximum, sum)
     float* listed;           // z of each list entry, [row][entries]
     float* loss;
     float* lse;
@@ -189,20 +189,17 @@ __device__ __forceinline__ uint32_t reversed(uint32_t x) {
     return y;
 }
 
-// The running maximum of a row and the sum of exp(z - maximum). The shift is
-// the scaled maximum as rounded, in powers of two; a sum of nothing but -inf
-// takes any finite shift.
+// The running maximum of a row and the sum of 2^((z - maximum) c); a sum of
+// nothing but -inf takes any finite maximum.
 struct Running {
-    float top = -INFINITY, shift = -INFINITY, sum = 0.0f;
+    float top = -INFINITY, sum = 0.0f;
 
     __device__ __forceinline__ void take(float z, float c) {
         if (z > top) {
-            const float to = z * c;
-            sum *= pow2(shift - to);
+            sum *= pow2((top - z) * c);
             top = z;
-            shift = to;
         }
-        sum += pow2(fmaf(z, c, top == -INFINITY ? 0.0f : -shift));
+        sum += pow2((z - (top == -INFINITY ? 0.0f : top)) * c);
     }
 };
 
@@ -254,8 +251,8 @@ __global__ void __launch_bounds__(kScoreThreads, 1) scoreFew(const ScoreParams p
     }
 #pragma unroll
     for (uint32_t o = T; o < T * kScoreAcross; o *= 2)
-        fold(run.shift, run.sum, __shfl_xor_sync(0xffffffffu, run.shift, o), __shfl_xor_sync(0xffffffffu, run.sum, o));
-    if (lane < T) parts[warp][reversed<T>(lane)] = make_float2(run.shift, run.sum);
+        fold(run.top, run.sum, __shfl_xor_sync(0xffffffffu, run.top, o), __shfl_xor_sync(0xffffffffu, run.sum, o), c);
+    if (lane < T) parts[warp][reversed<T>(lane)] = make_float2(run.top, run.sum);
 
     // z where a list (a label) names an entry of this class, a warp an entry.
     for (uint32_t e = at; e < p.rows * p.entries; e += of) {
@@ -273,7 +270,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1) scoreFew(const ScoreParams p
     if (threadIdx.x < T && threadIdx.x < p.rows) {
         float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (uint32_t k = 0; k < kScoreWarps; ++k) fold(top, sum, parts[k][threadIdx.x].x, parts[k][threadIdx.x].y);
+        for (uint32_t k = 0; k < kScoreWarps; ++k) fold(top, sum, parts[k][threadIdx.x].x, parts[k][threadIdx.x].y, c);
         p.strips[threadIdx.x * gridDim.x + blockIdx.x] = make_float2(top, sum);
     }
 }
@@ -296,10 +293,11 @@ __global__ void __launch_bounds__(kCloseThreads) closeFew(const ScoreParams p, u
         }
         return;
     }
+    const float c = p.scale * kLog2e;
     float top = -INFINITY, sum = 0.0f, target = 0.0f;
     for (uint32_t s = threadIdx.x; s < ctas; s += kCloseThreads) {
         const float2 x = p.strips[row * ctas + s];
-        fold(top, sum, x.x, x.y);
+        fold(top, sum, x.x, x.y, c);
     }
     for (uint32_t e = threadIdx.x; e < p.entries; e += kCloseThreads) {
         if (!p.labels && p.ids[row * p.entries + e] == kNoEntry) break;  // the list is sorted
@@ -309,7 +307,7 @@ __global__ void __launch_bounds__(kCloseThreads) closeFew(const ScoreParams p, u
     }
 #pragma unroll
     for (uint32_t o = 1; o < 32; o *= 2) {
-        fold(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
+        fold(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o), c);
         target += __shfl_xor_sync(0xffffffffu, target, o);
     }
     if (lane == 0) {
@@ -320,10 +318,10 @@ __global__ void __launch_bounds__(kCloseThreads) closeFew(const ScoreParams p, u
     __syncthreads();
     if (threadIdx.x == 0) {
         for (uint32_t w = 1; w < kWarps; ++w) {
-            fold(top, sum, tops[w], sums[w]);
+            fold(top, sum, tops[w], sums[w], c);
             target += targets[w];
         }
-        closeRow(row, top, sum, target, p.labels ? nullptr : p.entropy, p.loss, p.lse);
+        closeRow(row, top, sum, p.scale, target, p.labels ? nullptr : p.entropy, p.loss, p.lse);
     }
 }
 
