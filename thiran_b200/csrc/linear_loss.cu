@@ -55,8 +55,12 @@ using namespace thb::tc;
 constexpr uint32_t kBM = 128, kBN = 256, kBK = 64;
 constexpr uint32_t kListWarps = 2;  // that look up the targets of a tile's rows ahead of its read-out
 constexpr uint32_t kTmemCols = 512;
-// Products that the tensor cores sum before the read-out adds: 1024. Over
-// 4096 of them lse was 1.3e-6 of itself off, over 1024 4e-7.
+// Products of a logit that the tensor cores sum before the read-out adds: 1024.
+// They cut each addition, towards zero. Over 4096 products lse was 1.3e-6 of
+// itself off, over 1024 4e-7. The slopes add up their logits the same way, bit
+// for bit those that lse was made of: exp(z - lse) of a well-known label is 1
+// less a small rest, which a z with roundings of its own would drown (4096
+// products, logits around 40: off by 2e-4 where 1e-4 was right).
 constexpr uint32_t kBlocksPerSum = 16;
 constexpr uint32_t kABytes = kBM * kBK * 2;
 
@@ -64,38 +68,50 @@ enum : int {
     kEpiLse = 0,    // running (max, sum) of each row's strip, z at the listed columns
     kEpiSlope = 1,  // bf16 slopes of the loss
     kEpiTwin = 2,   // the same of few rows, and behind them what their rounding left
-    kEpiAcc = 3,    // f32, stored or added to C
-    kEpiOut = 4,    // bf16, rows optionally scattered by a map
+    kEpiSlopeSums = 3,  // both of logits that take more than one accumulator's sum
+    kEpiTwinSums = 4,
+    kEpiAcc = 5,    // f32, stored or added to C
+    kEpiOut = 6,    // bf16, rows optionally scattered by a map
 };
 
-constexpr bool givesSlopes(int epilogue) { return epilogue == kEpiSlope || epilogue == kEpiTwin; }
+constexpr bool givesTwins(int epilogue) { return epilogue == kEpiTwin || epilogue == kEpiTwinSums; }
+constexpr bool givesSlopes(int epilogue) { return epilogue == kEpiSlope || epilogue == kEpiSlopeSums || givesTwins(epilogue); }
 constexpr bool usesLists(int epilogue) { return epilogue == kEpiLse || givesSlopes(epilogue); }
+constexpr bool sumsLogits(int epilogue) {
+    return epilogue == kEpiLse || epilogue == kEpiSlopeSums || epilogue == kEpiTwinSums;
+}
 
 // Epilogue warps: two per TMEM lane quadrant, which split the tile's columns;
-// four for lse, whose part of a row then fits in 64 registers. (A 1024 x
-// 37888 pass: 33.5 -> 29.3 us at a width of 256, 68 -> 66.5 at 1024. The
-// slopes' staging blocks for four would cost the ring a stage: 38.5 -> 36 us,
-// but 67.8 -> 69.)
-constexpr uint32_t epilogueWarps(int epilogue) { return epilogue == kEpiLse ? 16 : 8; }
+// four for logits that are summed, whose part of a row then fits in 64
+// registers. (lse: a 1024 x 37888 pass 33.5 -> 29.3 us at a width of 256, 68 ->
+// 66.5 at 1024. Slopes of one accumulator are read out faster by two: gradients
+// of 64 rows, 32768 x 1024, 65 us against 68. Those of several, with 128 sums a
+// thread of which most lie in local memory, are not: 2048 rows, 65536 x 2048,
+// 1235 us by two, 1146 by four.)
+constexpr uint32_t epilogueWarps(int epilogue) { return sumsLogits(epilogue) ? 16 : 8; }
 constexpr uint32_t partsFor(int epilogue) { return epilogueWarps(epilogue) / 4; }
 constexpr uint32_t partColumns(int epilogue) { return kBN / partsFor(epilogue); }
 constexpr uint32_t threadsFor(int epilogue) {
     return 64 + 32 * (epilogueWarps(epilogue) + (usesLists(epilogue) ? kListWarps : 0));
 }
-constexpr uint32_t kLseParts = partsFor(kEpiLse);
+constexpr uint32_t kLogitParts = partsFor(kEpiLse);  // at most
 // Strips of a row in a tile of lse.
 __host__ __device__ constexpr uint32_t stripsOf(uint32_t tileN) {
-    return (tileN + kBN / kLseParts - 1) / (kBN / kLseParts);
+    return (tileN + kBN / kLogitParts - 1) / (kBN / kLogitParts);
 }
 
-// Rows of the read-out's staging blocks: 64 bytes and a shift of the banks.
-constexpr uint32_t kStageLd = 80;
-constexpr bool stagesOutput(int epilogue) { return givesSlopes(epilogue) || epilogue == kEpiOut; }
+// Rows of the read-out's staging blocks: 64 bytes and a shift of the banks, or
+// (four warps a quadrant, whose blocks must leave the ring its stages) 32 bytes.
+constexpr uint32_t kStageLd = 80, kSlopeStageLd = 32;
+constexpr uint32_t stageLdFor(int epilogue) {
+    if (epilogue == kEpiLse || epilogue == kEpiAcc) return 0;
+    return sumsLogits(epilogue) ? kSlopeStageLd : kStageLd;
+}
 
 // What the read-out of a logits tile needs of its rows: the list's place and,
 // for each part of the columns, its first entry there.
 struct TileRows {
-    uint32_t at[kLseParts][kBM], next[kLseParts][kBM], row[kBM];
+    uint32_t at[kLogitParts][kBM], next[kLogitParts][kBM], row[kBM];
     float minusLse[kBM], scale[kBM];  // scale: scale * grad_loss
 };
 
@@ -106,7 +122,7 @@ struct Geometry {
     static constexpr uint32_t bBytes = bRows * kBK * 2;
     static constexpr uint32_t stageBytes = kABytes + bBytes;
     static constexpr uint32_t tileM = PAIR ? 2 * kBM : kBM;
-    static constexpr uint32_t blockBytes = stagesOutput(EPI) ? epilogueWarps(EPI) * 32 * kStageLd : 0;
+    static constexpr uint32_t blockBytes = epilogueWarps(EPI) * 32 * stageLdFor(EPI);
     static constexpr uint32_t smemBytes =
         stages * stageBytes + blockBytes + (usesLists(EPI) ? 2 * sizeof(TileRows) : 0) + 1024;
     static_assert(smemBytes + 512 <= 232448, "shared memory");
@@ -126,7 +142,7 @@ struct Params {
     uint32_t countIsM, countIsK;
     uint32_t m, n, k;
     uint32_t nTiles, splits, blocksPerSplit;  // k blocks of a split (splits > 1 only with a fixed k)
-    uint32_t blocksPerSum;                    // kEpiLse: k blocks that one accumulator sums
+    uint32_t blocksPerSum;                    // sumsLogits: k blocks that one accumulator sums
     uint32_t aRows;                           // rows of a loaded block of A (K-major A; fewer than 128: the rest is not used)
     uint32_t tileN;                           // columns of a tile (K-major B): 32 to 256, a multiple of 32
     uint32_t group;                           // m blocks per raster group
@@ -245,6 +261,36 @@ __device__ __forceinline__ void storeBf16Block(uint8_t* stage, __nv_bfloat16* c,
     }
 }
 
+// The same of 16 columns of slopes, whose rows lie at 32-byte boundaries: a
+// store instruction writes 16 sectors. The halves of a staged row change places
+// every four rows, so that eight rows' halves meet every bank once.
+__device__ __forceinline__ void storeSlopes(uint8_t* stage, __nv_bfloat16* c, uint64_t ldc, uint32_t row, uint32_t rows,
+                                            uint32_t col, const float (&v)[16], uint32_t lane) {
+    uint4* block = reinterpret_cast<uint4*>(stage);
+    __syncwarp();  // the block before has been read
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        uint4 packed;
+        __nv_bfloat162* pairs = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) pairs[e] = __floats2bfloat162_rn(v[h * 8 + 2 * e], v[h * 8 + 2 * e + 1]);
+        block[lane * 2 + (h ^ (lane / 4 % 2))] = packed;
+    }
+    __syncwarp();
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t r = i * 16 + lane / 2, h = lane % 2;
+        const uint4 packed = block[r * 2 + (h ^ (r / 4 % 2))];
+        if (r < rows) *reinterpret_cast<uint4*>(c + static_cast<uint64_t>(row - lane + r) * ldc + col + h * 8) = packed;
+    }
+}
+
+// The same of 32 columns, through rows of kStageLd.
+__device__ __forceinline__ void storeSlopes(uint8_t* stage, __nv_bfloat16* c, uint64_t ldc, uint32_t row, uint32_t rows,
+                                            uint32_t col, const float (&v)[32], uint32_t lane) {
+    storeBf16Block<false>(stage, c, ldc, row, rows, col, v, 32u, lane);
+}
+
 // The tiles first, first + step, ... of one matrix of products, by a CTA or a
 // pair.
 template <bool A_MN, bool B_MN, int EPI, bool PAIR>
@@ -258,7 +304,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
     __shared__ __align__(8) uint64_t rowsFull[2], rowsEmpty[2];
     __shared__ uint32_t tmemSlot;
     __shared__ volatile int abortFlag;
-    __shared__ float2 parts[kLseParts][32];  // of the rows' strips, and
+    __shared__ float2 parts[kLogitParts][32];  // of the rows' strips, and
     __shared__ bool lastOne;                 // whether this CTA joins them (finished)
     (void)parts;
     (void)lastOne;
@@ -411,7 +457,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                 bool ok = true;
                 uint32_t kb = kb0;
                 do {  // one accumulator: the whole k range, or blocksPerSum of it
-                    const uint32_t end = EPI == kEpiLse ? min(kb + p.blocksPerSum, kb1) : kb1;
+                    const uint32_t end = sumsLogits(EPI) ? min(kb + p.blocksPerSum, kb1) : kb1;
                     if (!mbarWait(&tmemEmpty[acc], accPhase ^ 1u, &abortFlag)) { abortFlag = 1; ok = false; break; }
                     fenceAfter();
                     const uint32_t d = tmemBase + acc * kBN;
@@ -518,7 +564,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
         const uint32_t quadrant = warp % 4;  // TMEM lanes 32 * quadrant .. + 31
         const uint32_t part = (warp - 2) / 4;
         uint32_t acc = 0, accPhase = 0;
-        uint8_t* stage = base + G::stages * G::stageBytes + (warp - 2) * 32 * kStageLd;
+        uint8_t* stage = base + G::stages * G::stageBytes + (warp - 2) * 32 * stageLdFor(EPI);
         (void)stage;
         uint32_t rowsBuf = 0, rowsPhase = 0;
         float runningTop = -INFINITY, runningSum = 0.0f;
@@ -567,38 +613,102 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                 else mbarArrive(&tmemEmpty[acc]);
                 if (++acc == 2) { acc = 0; accPhase ^= 1u; }
             };
-            if constexpr (EPI == kEpiLse) {
+            // Logits of a row, from `col` of C on, to slopes in memory.
+            auto giveSlopes = [&](auto& v, uint32_t col) {
+                constexpr uint32_t kWidth = sizeof(v) / sizeof(v[0]);
+                const float2 slope2 = make_float2(rowScale, rowScale), scale2 = make_float2(p.scale, p.scale);
+#pragma unroll
+                for (uint32_t j = 0; j < kWidth; j += 2) {
+                    const float2 e = mul2(slope2, pow2Shifted(mul2(make_float2(v[j], v[j + 1]), scale2), minusLse, kLog2e));
+                    v[j] = e.x;
+                    v[j + 1] = e.y;
+                }
+                while (next < p.bFirstN + col + kWidth) {
+                    const float share = rowScale * (p.shares ? p.shares[list + at] : 1.0f);
+                    const uint32_t j0 = next - (p.bFirstN + col);
+#pragma unroll
+                    for (uint32_t j = 0; j < kWidth; ++j) v[j] = __fsub_rn(v[j], j0 == j ? share : 0.0f);
+                    next = ++at < p.entries ? ids[at] : kNoEntry;
+                }
+                // Rows and columns behind the last are operands of the next
+                // products (whole k blocks): zeros.
+                const uint32_t left = p.n > col ? p.n - col : 0u;  // columns of v inside C
+                if (rowsHere < 32 || left < kWidth) {
+#pragma unroll
+                    for (uint32_t j = 0; j < kWidth; ++j)
+                        if (!live || j >= left) v[j] = 0.0f;
+                }
+                // The slopes are rounded to bf16, the tensor cores' operand
+                // type: as much as the gradients' own rounding. Where few rows
+                // leave the tile room, what the rounding left follows as rows
+                // of its own, whose products add to the same sums: the few
+                // slopes that such gradients consist of do not average their
+                // roundings out. (64 rows, 32768 x 2048: off by 0.0017 of the
+                // norm instead of 0.0024, 148 us a step instead of 140.)
+                __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.c);
+                if constexpr (!givesTwins(EPI)) {
+                    storeSlopes(stage, c, p.ldc, row, 32u, col, v, lane);
+                } else {
+                    uint32_t to = row, end = p.twin;
+#pragma unroll 1
+                    for (;;) {
+                        if (row - lane < end) storeSlopes(stage, c, p.ldc, to, min(end - (row - lane), 32u), col, v, lane);
+                        if (to != row) break;
+#pragma unroll
+                        for (uint32_t j = 0; j < kWidth; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+                        to = row + p.twin;
+                        end = kBM - p.twin;
+                    }
+                }
+            };
+            (void)giveSlopes;
+            if constexpr (sumsLogits(EPI)) {
                 // The strip of a row, in registers. The tensor cores cut each
                 // addition to f32, which over a long k drifts towards zero;
                 // sums over blocksPerSum k blocks are added here, rounded.
                 uint32_t raw[kStrip / 32][32];
                 auto z = [&](uint32_t j) { return __uint_as_float(raw[j / 32][j % 32]); };
-                bool ok = true;
-                for (uint32_t kb = 0; kb < kBlocks; kb += p.blocksPerSum) {
+                auto arrived = [&] {  // (The warp leaves together.)
                     if (!mbarWait(&tmemFull[acc], accPhase, &abortFlag)) abortFlag = 1;
-                    if (__any_sync(0xffffffffu, abortFlag)) { ok = false; break; }  // the warp leaves together
+                    if (__any_sync(0xffffffffu, abortFlag)) return false;
                     fenceAfter();
-                    const uint32_t columns = tmemBase + ((quadrant * 32u) << 16) + acc * kBN + part * kStrip;
-                    if (kb == 0) {
+                    return true;
+                };
+                const uint32_t columns = tmemBase + ((quadrant * 32u) << 16) + part * kStrip;
+                if (!arrived()) break;
 #pragma unroll
-                        for (uint32_t q = 0; q < kStrip / 32; ++q) tmemFetch32(columns + q * 32u, raw[q]);
+                for (uint32_t q = 0; q < kStrip / 32; ++q) tmemFetch32(columns + acc * kBN + q * 32u, raw[q]);
 #pragma unroll
-                        for (uint32_t q = 0; q < kStrip / 32; ++q) tmemArrived(raw[q]);
-                    } else {
+                for (uint32_t q = 0; q < kStrip / 32; ++q) tmemArrived(raw[q]);
+                release();
+                bool ok = true;
+                for (uint32_t kb = p.blocksPerSum; kb < kBlocks; kb += p.blocksPerSum) {
+                    if (!(ok = arrived())) break;
 #pragma unroll
-                        for (uint32_t q = 0; q < kStrip / 16; ++q) {
-                            uint32_t r[16];
-                            tmemLoad16(columns + q * 16u, r);
+                    for (uint32_t q = 0; q < kStrip / 16; ++q) {
+                        uint32_t r[16];
+                        tmemLoad16(columns + acc * kBN + q * 16u, r);
 #pragma unroll
-                            for (uint32_t j = 0; j < 16; ++j) {
-                                uint32_t& sum = raw[q / 2][q % 2 * 16 + j];
-                                sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(r[j]));
-                            }
+                        for (uint32_t j = 0; j < 16; ++j) {
+                            uint32_t& sum = raw[q / 2][q % 2 * 16 + j];
+                            sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(r[j]));
                         }
                     }
                     release();
                 }
                 if (!ok) break;
+                if constexpr (givesSlopes(EPI)) {
+#pragma unroll
+                    for (uint32_t q = 0; q < kStrip / 16; ++q) {
+                        const uint32_t col = col0 + q * 16;
+                        if (q * 16 >= width || col >= p.ldc) break;
+                        float v[16];
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; ++j) v[j] = z(q * 16 + j);
+                        giveSlopes(v, col);
+                    }
+                    continue;
+                }
                 if (!live || width == 0) continue;
                 const uint32_t left = p.n > col0 ? min(p.n - col0, width) : 0u;  // columns of the strip in the vocabulary
                 if (left < kStrip) {
@@ -653,51 +763,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                 else release();
                 const uint32_t left = p.n > col ? p.n - col : 0u;  // columns of the chunk inside C
                 if constexpr (givesSlopes(EPI)) {
-                    const float2 slope2 = make_float2(rowScale, rowScale), scale2 = make_float2(p.scale, p.scale);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float2 e = mul2(slope2, pow2Shifted(mul2(make_float2(v[j], v[j + 1]), scale2), minusLse, kLog2e));
-                        v[j] = e.x;
-                        v[j + 1] = e.y;
-                    }
-                    while (next < p.bFirstN + col + 32) {
-                        const float share = rowScale * (p.shares ? p.shares[list + at] : 1.0f);
-                        const uint32_t j0 = next - (p.bFirstN + col);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __fsub_rn(v[j], j0 == static_cast<uint32_t>(j) ? share : 0.0f);
-                        next = ++at < p.entries ? ids[at] : kNoEntry;
-                    }
-                    // Rows and columns behind the last are operands of the
-                    // next products (whole k blocks): zeros.
-                    if (rowsHere < 32 || left < 32) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!live || j >= static_cast<int>(left)) v[j] = 0.0f;
-                    }
-                    // The slopes are rounded to bf16, the tensor cores' operand
-                    // type: as much as the gradients' own rounding. Where few
-                    // rows leave the tile room, what the rounding left follows
-                    // as rows of its own, whose products add to the same sums:
-                    // the few slopes that such gradients consist of do not
-                    // average their roundings out. (64 rows, 32768 x 2048: off
-                    // by 0.0017 of the norm instead of 0.0024, 148 us a step
-                    // instead of 140.)
-                    __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.c);
-                    if constexpr (EPI == kEpiSlope) {
-                        storeBf16Block<false>(stage, c, p.ldc, row, 32u, col, v, 32u, lane);
-                    } else {
-                        uint32_t to = row, end = p.twin;
-#pragma unroll 1
-                        for (;;) {
-                            if (row - lane < end)
-                                storeBf16Block<false>(stage, c, p.ldc, to, min(end - (row - lane), 32u), col, v, 32u, lane);
-                            if (to != row) break;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
-                            to = row + p.twin;
-                            end = kBM - p.twin;
-                        }
-                    }
+                    giveSlopes(v, col);
                 } else {
                     if (kBlocks == 0) {
 #pragma unroll
@@ -1399,7 +1465,7 @@ cudaError_t gemm(const CUtensorMap& a, const CUtensorMap& b, Params& p, uint64_t
     p.group = 16;
     const uint64_t tiles = (maxM + tileM - 1) / tileM * p.nTiles * p.splits;
     if (tiles > UINT32_MAX / 2) return cudaErrorInvalidValue;
-    if constexpr (EPI != kEpiTwin) {  // (its rows fit half a CTA's)
+    if constexpr (!givesTwins(EPI)) {  // (its rows fit half a CTA's)
         if (pair) return launchTyped<A_MN, B_MN, EPI, true>(a, b, p, tiles, smCount, stream);
     }
     return launchTyped<A_MN, B_MN, EPI, false>(a, b, p, tiles, smCount, stream);
@@ -1797,8 +1863,13 @@ cudaError_t backward(const Problem& q, int smCount, std::uint32_t* status, cudaS
         s.twin = l.twin;
         s.c = slopes;
         s.ldc = l.piece;
-        e = l.twin ? gemm<false, false, kEpiTwin>(hiddenK, weightK, s, q.rows, false, smCount, stream)
-                   : gemm<false, false, kEpiSlope>(hiddenK, weightK, s, q.rows, pair, smCount, stream);
+        s.blocksPerSum = kBlocksPerSum;
+        if (q.dim <= kBlocksPerSum * kBK)
+            e = l.twin ? gemm<false, false, kEpiTwin>(hiddenK, weightK, s, q.rows, false, smCount, stream)
+                       : gemm<false, false, kEpiSlope>(hiddenK, weightK, s, q.rows, pair, smCount, stream);
+        else
+            e = l.twin ? gemm<false, false, kEpiTwinSums>(hiddenK, weightK, s, q.rows, false, smCount, stream)
+                       : gemm<false, false, kEpiSlopeSums>(hiddenK, weightK, s, q.rows, pair, smCount, stream);
         if (e != cudaSuccess) return e;
         Params h = base;
         h.countIsM = !l.twin;
