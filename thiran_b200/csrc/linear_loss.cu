@@ -15,7 +15,8 @@
 //             and stores z where a list names the column; the strips are
 //             then folded into log-sum-exp and loss. (A few rows go to
 //             linear_score.cuh instead, without packing or tensor cores.)
-//   backward  for each piece of the vocabulary: the logits again, whose
+//   backward  for each piece of the vocabulary: the logits again (summed as
+//             the forward pass sums them, by the same kernels), whose
 //             epilogue turns them into the slopes
 //             G = scale * grad_loss * (exp(z - lse) - share) in bf16 (of up
 //             to 64 rows in two bf16 summands); then
@@ -1508,7 +1509,7 @@ struct Layout {
     uint32_t twin;           // rows of slopes, and behind them as many of what their rounding left; 0: one
     bool direct;             // dH in one go, straight to its rows
     uint32_t hiddenUnits;    // CTAs or pairs for dH, dW on the others; 0: one after the other
-    uint32_t scoreCtas;      // of scoreFew; 0: the products go to the tensor cores
+    uint32_t scoreCtas;      // of scoreFew, both passes; 0: the logits go to the tensor cores
     uint64_t count, rowMap, rowScale, rowLse, state, ids, shares, entropy, packed, weights;
     uint64_t strips, listed;  // forward
     uint64_t slopes, acc;     // backward (shares the forward's place)
@@ -1603,7 +1604,7 @@ Layout layoutFor(uint64_t rows, uint64_t vocab, uint64_t dim, uint64_t entries, 
     l.stripCount = (vocab + l.tileN - 1) / l.tileN * stripsOf(l.tileN);
     l.splits = 1;
     if (backward) planGradients(l, rows, std::min(l.piece, vocab), dim, mTiles, slots, pair);
-    if (!backward) l.scoreCtas = scoreCtas(rows, vocab, dim, aligned, smCount);
+    l.scoreCtas = scoreCtas(rows, vocab, dim, aligned, smCount);
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -1619,7 +1620,7 @@ Layout layoutFor(uint64_t rows, uint64_t vocab, uint64_t dim, uint64_t entries, 
     l.shares = take(rows * entries * 4);
     l.entropy = take(rows * 4);
     l.packed = take(l.rowsPad * l.dimPad * 2);
-    l.weights = take(aligned || l.scoreCtas ? 0 : vocab * l.dimPad * 2);
+    l.weights = take(aligned || (l.scoreCtas && !backward) ? 0 : vocab * l.dimPad * 2);
     const uint64_t shared = at;
     l.strips = take(l.stripCount * l.rowsPad * 8);  // more than scoreFew's, at most 8 a 16 rows of weights
     l.listed = take(rows * entries * 4);
@@ -1716,21 +1717,27 @@ cudaError_t plan(const Problem& q, const Layout& l, bool backward, int smCount, 
     return e;
 }
 
-template <uint32_t T>
-cudaError_t launchScore(const ScoreParams& p, uint32_t ctas, cudaStream_t stream) {
+template <uint32_t T, bool SLOPES>
+cudaError_t launchScoreRows(const ScoreParams& p, uint32_t ctas, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};
-    const cudaError_t e = allowShared(scoreFew<T>, kScoreShared, ready);
+    const cudaError_t e = allowShared(scoreFew<T, SLOPES>, kScoreShared, ready);
     if (e != cudaSuccess) return e;
-    return launch(scoreFew<T>, ctas, kScoreThreads, static_cast<uint32_t>(T * scoreLd(p.dim) * 4), stream, 1, p);
+    return launch(scoreFew<T, SLOPES>, ctas, kScoreThreads, static_cast<uint32_t>(T * scoreLd(p.dim) * 4), stream, 1, p);
 }
 
-cudaError_t score(const Problem& q, const Layout& l, uint32_t* status, cudaStream_t stream) {
-    cudaError_t e = cudaSuccess;
-    if (!q.labels) e = teacher(q, l, Align{}, 0, status, stream);
-    if (e != cudaSuccess) return e;
+template <bool SLOPES>
+cudaError_t launchScore(const ScoreParams& p, uint32_t ctas, cudaStream_t stream) {
+    switch (scoreHeight(p.rows)) {
+    case 1: return launchScoreRows<1, SLOPES>(p, ctas, stream);
+    case 2: return launchScoreRows<2, SLOPES>(p, ctas, stream);
+    case 4: return launchScoreRows<4, SLOPES>(p, ctas, stream);
+    default: return launchScoreRows<8, SLOPES>(p, ctas, stream);
+    }
+}
+
+// What both passes of a few rows share.
+ScoreParams scoreParams(const Problem& q, const Layout& l, uint32_t* status) {
     ScoreParams p{};
-    p.hidden = static_cast<const __nv_bfloat16*>(q.hidden);
-    p.ldHidden = q.ldHidden;
     p.weight = static_cast<const __nv_bfloat16*>(q.weight);
     p.ldWeight = q.ldWeight;
     p.rows = static_cast<uint32_t>(q.rows);
@@ -1740,23 +1747,28 @@ cudaError_t score(const Problem& q, const Layout& l, uint32_t* status, cudaStrea
     p.classes = 8;
     while (p.classes > 1 && q.ldWeight * p.classes / 2 % 8 == 0) p.classes /= 2;
     p.scale = q.scale;
+    p.ids = place<uint32_t>(q, l.ids);
+    p.shares = q.labels ? nullptr : place<float>(q, l.shares);
+    p.status = status;
+    return p;
+}
+
+cudaError_t score(const Problem& q, const Layout& l, uint32_t* status, cudaStream_t stream) {
+    cudaError_t e = cudaSuccess;
+    if (!q.labels) e = teacher(q, l, Align{}, 0, status, stream);
+    if (e != cudaSuccess) return e;
+    ScoreParams p = scoreParams(q, l, status);
+    p.hidden = static_cast<const __nv_bfloat16*>(q.hidden);
+    p.ldHidden = q.ldHidden;
     p.labels = q.labels;
     p.ignore = q.ignore;
     p.state = place<uint8_t>(q, l.state);
-    p.ids = place<uint32_t>(q, l.ids);
-    p.shares = place<float>(q, l.shares);
     p.entropy = place<float>(q, l.entropy);
     p.strips = place<float2>(q, l.strips);
     p.listed = place<float>(q, l.listed);
     p.loss = q.loss;
     p.lse = q.lse;
-    p.status = status;
-    switch (scoreHeight(q.rows)) {
-    case 1: e = launchScore<1>(p, l.scoreCtas, stream); break;
-    case 2: e = launchScore<2>(p, l.scoreCtas, stream); break;
-    case 4: e = launchScore<4>(p, l.scoreCtas, stream); break;
-    default: e = launchScore<8>(p, l.scoreCtas, stream);
-    }
+    e = launchScore<false>(p, l.scoreCtas, stream);
     if (e != cudaSuccess) return e;
     return launch(closeFew, p.rows, kCloseThreads, 0, stream, 1, p, l.scoreCtas);
 }
@@ -1838,7 +1850,8 @@ cudaError_t backward(const Problem& q, int smCount, std::uint32_t* status, cudaS
         !makeMap(&weightK, weight, q.dim, q.vocab, ldWeight, pair ? l.pieceTileN / 2 : l.pieceTileN) ||
         !makeMap(&slopesK, slopes, l.piece, l.rowsPad, l.piece, blockRows(slopeRows)) ||
         !makeMap(&weightMN, weight, q.dim, q.vocab, ldWeight, 64) ||
-        !makeMap(&slopesMN, slopes, l.piece, l.rowsPad, l.piece, 64) ||
+        // (scoreFew writes the rows of both summands; those behind are read as zeros.)
+        !makeMap(&slopesMN, slopes, l.piece, l.scoreCtas ? slopeRows : l.rowsPad, l.piece, 64) ||
         !makeMap(&hiddenMN, packed, l.dimPad, l.rowsPad, l.dimPad, 64))
         return cudaErrorInvalidValue;
     Params base{};
@@ -1864,7 +1877,21 @@ cudaError_t backward(const Problem& q, int smCount, std::uint32_t* status, cudaS
         s.c = slopes;
         s.ldc = l.piece;
         s.blocksPerSum = kBlocksPerSum;
-        if (q.dim <= kBlocksPerSum * kBK)
+        if (l.scoreCtas) {  // (up to kScoreRows rows: their twins are as many on)
+            ScoreParams f = scoreParams(q, l, status);
+            f.hidden = static_cast<const __nv_bfloat16*>(packed);
+            f.ldHidden = l.dimPad;
+            f.weight += first * q.ldWeight;
+            f.vocab = static_cast<uint32_t>(width);
+            f.first = static_cast<uint32_t>(first);
+            f.count = base.count;
+            f.rowMap = s.rowMap;
+            f.rowLse = s.rowLse;
+            f.rowScale = s.rowScale;
+            f.slopes = static_cast<__nv_bfloat16*>(slopes);
+            f.ldSlopes = l.piece;
+            e = launchScore<true>(f, l.scoreCtas, stream);
+        } else if (q.dim <= kBlocksPerSum * kBK)
             e = l.twin ? gemm<false, false, kEpiTwin>(hiddenK, weightK, s, q.rows, false, smCount, stream)
                        : gemm<false, false, kEpiSlope>(hiddenK, weightK, s, q.rows, pair, smCount, stream);
         else

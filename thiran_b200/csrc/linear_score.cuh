@@ -1,5 +1,5 @@
-// lse and loss of a few rows (a token at a time, a short batch): the forward
-// pass of the linear losses without tensor cores.
+// lse and loss of a few rows (a token at a time, a short batch), and their
+// slopes: the logits of the linear losses without tensor cores.
 //
 // Up to kScoreRows rows the products are small beside the weights that they
 // read, so that the weights are streamed once through plain loads, each
@@ -8,6 +8,12 @@
 // every row. No packing and no copies: rows of weights at any address are read
 // in the aligned 16-byte vectors that hold them, against H shifted as far. Rows
 // with the same shift are `classes` apart; a CTA takes those of one class.
+//
+// The slopes of rows that were scored here are computed here too, from the same
+// sums: exp(z - lse) of a well-known label is 1 less a small rest, which the
+// tensor cores' roundings of z would drown (8 rows of 4096 products, logits
+// around 40: off by 5e-5 where 1e-4 was right). They are written as the tensor
+// cores' kernel writes those of few rows, in two bf16 summands.
 //
 // Against the tensor cores' path, us a call in a graph (whose weights stay in
 // L2 where they fit): 1 row, 32768 x 1024 11.6 to 17.9, 4 rows 17.7 to 18.3;
@@ -50,6 +56,15 @@ struct ScoreParams {
     float* loss;
     float* lse;
     uint32_t* status;
+    // Slopes: `weight` and `vocab` are those of a piece of the vocabulary, from
+    // entry `first` (a multiple of 8) on; `hidden` is packed.
+    uint32_t first;
+    const uint32_t* count;   // packed rows
+    const uint32_t* rowMap;  // packed row -> row
+    const float* rowLse;     // packed
+    const float* rowScale;   // packed: scale * grad_loss
+    __nv_bfloat16* slopes;   // [2 kScoreRows][ldSlopes], what the roundings left behind the slopes
+    uint64_t ldSlopes;
 };
 
 __device__ __forceinline__ uint8_t stateOf(const ScoreParams& p, uint32_t row) {
@@ -203,7 +218,72 @@ struct Running {
     }
 };
 
-template <uint32_t T>
+// What a lane knows of the row of H whose slopes it gives: the place in its
+// list from the current entry of the vocabulary on.
+struct SlopeRow {
+    float lse = 0.0f, scale = 0.0f;
+    uint64_t list = 0;
+    uint32_t at = 0, next = kNoEntry;
+    bool live = false;
+
+    __device__ __forceinline__ void step(const ScoreParams& p) {
+        next = ++at < p.entries ? p.ids[list + at] : kNoEntry;
+    }
+
+    // The list's first entry from `entry` on.
+    __device__ __forceinline__ void begin(const ScoreParams& p, uint32_t row, uint32_t rows, uint32_t entry) {
+        live = row < rows;
+        if (!live) return;
+        lse = p.rowLse[row];
+        scale = p.rowScale[row];
+        list = static_cast<uint64_t>(p.rowMap[row]) * p.entries;
+        uint32_t end = p.entries;
+        while (at < end) {
+            const uint32_t middle = (at + end) / 2;
+            if (p.ids[list + middle] < entry) at = middle + 1;
+            else end = middle;
+        }
+        next = at < p.entries ? p.ids[list + at] : kNoEntry;
+    }
+
+    // The slope at z (unscaled) of `entry`, rounded as in the tensor cores' kernel.
+    __device__ __forceinline__ float take(const ScoreParams& p, float z, uint32_t entry) {
+        float slope = __fmul_rn(scale, pow2(__fmul_rn(__fadd_rn(__fmul_rn(z, p.scale), -lse), kLog2e)));
+        while (next < entry) step(p);
+        while (next == entry) {
+            slope = __fsub_rn(slope, scale * (p.shares ? p.shares[list + at] : 1.0f));
+            step(p);
+        }
+        return slope;
+    }
+};
+
+// `slope` of packed row `row` in two summands at column v.
+__device__ __forceinline__ void giveSlope(const ScoreParams& p, uint32_t row, uint32_t v, float slope) {
+    const __nv_bfloat16 high = __float2bfloat16_rn(slope);
+    p.slopes[row * p.ldSlopes + v] = high;
+    p.slopes[(row + kScoreRows) * p.ldSlopes + v] = __float2bfloat16_rn(slope - __bfloat162float(high));
+}
+
+// The slopes behind those of the packed rows are operands of the next products:
+// zeros, in rows up to kScoreRows and in columns up to the end of a k block of
+// 64. A CTA fills a run of 16-byte vectors in each row.
+__device__ __forceinline__ void zeroSlopes(const ScoreParams& p, uint32_t packed) {
+    const uint32_t vectors = (p.vocab + 63) / 64 * 8;
+    const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(vectors) * blockIdx.x / gridDim.x);
+    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(vectors) * (blockIdx.x + 1) / gridDim.x);
+    for (uint32_t row = packed; row < 2 * kScoreRows; ++row) {
+        if (row % kScoreRows < packed) continue;
+        uint4* to = reinterpret_cast<uint4*>(p.slopes + row * p.ldSlopes);
+        for (uint32_t i = first + threadIdx.x; i < end; i += kScoreThreads) to[i] = make_uint4(0, 0, 0, 0);
+    }
+    const uint32_t behind = (p.vocab + 63) / 64 * 64 - p.vocab;
+    if (blockIdx.x == 0)
+        for (uint32_t e = threadIdx.x; e < packed * behind; e += kScoreThreads)
+            giveSlope(p, e / behind, p.vocab + e % behind, 0.0f);
+}
+
+template <uint32_t T, bool SLOPES>
 __global__ void __launch_bounds__(kScoreThreads, 1) scoreFew(const ScoreParams p) {
     extern __shared__ float4 sharedHidden[];
     __shared__ float2 parts[kScoreWarps][T];
@@ -217,12 +297,14 @@ __global__ void __launch_bounds__(kScoreThreads, 1) scoreFew(const ScoreParams p
     const auto vectorsAt = [&](uint32_t v) { return reinterpret_cast<const uint4*>(rowAt(v) - off); };
     gridDependencyLaunch();
     gridDependencyWait();
-    const bool mine = threadIdx.x < p.rows && stateOf(p, threadIdx.x) == kLive;
-#pragma unroll
-    for (uint32_t t = 0; t < T; ++t)
-        fillRow(h + t * ldh, t < p.rows ? p.hidden + t * p.ldHidden : nullptr, p.dim, off, vectors);
     // Without a target no row needs the weights.
-    if (!__syncthreads_or(mine)) return;
+    const uint32_t packed = SLOPES ? *p.count : 0u;
+    if (SLOPES && packed == 0) return;
+    const bool mine = !SLOPES && threadIdx.x < p.rows && stateOf(p, threadIdx.x) == kLive;
+#pragma unroll
+    for (uint32_t t = 0; t < T; ++t)  // (packed rows: zeros behind the last)
+        fillRow(h + t * ldh, SLOPES || t < p.rows ? p.hidden + t * p.ldHidden : nullptr, p.dim, off, vectors);
+    if (!__syncthreads_or(mine) && !SLOPES) return;
 
     // A run of them for each warp.
     const uint32_t at = blockIdx.x / p.classes * kScoreWarps + warp;
@@ -233,6 +315,9 @@ __global__ void __launch_bounds__(kScoreThreads, 1) scoreFew(const ScoreParams p
     const float c = p.scale * kLog2e;
     // Lane l holds row reversed<T>(l) of H, of weight rows reversed<kScoreAcross>(l / T).
     Running run;
+    SlopeRow row;
+    const uint32_t t = reversed<T>(lane);
+    if constexpr (SLOPES) row.begin(p, t, packed, p.first + own + i * p.classes);
     for (; i + kScoreAcross <= end; i += kScoreAcross) {
         const uint4* w[kScoreAcross];
 #pragma unroll
@@ -240,29 +325,43 @@ __global__ void __launch_bounds__(kScoreThreads, 1) scoreFew(const ScoreParams p
         float z[T * kScoreAcross];
         dots<T>(w, h, ldh, p.dim, off, lane, z);
         const float x = warpSums(z, lane);
-        if (lane < T * kScoreAcross) run.take(x, c);
+        if constexpr (SLOPES) {
+            const uint32_t v = own + (i + reversed<kScoreAcross>(lane / T)) * p.classes;
+            if (lane < T * kScoreAcross && row.live) giveSlope(p, t, v, row.take(p, x, p.first + v));
+        } else {
+            if (lane < T * kScoreAcross) run.take(x, c);
+        }
     }
     for (; i < end; ++i) {
-        const uint4* const w[1] = {vectorsAt(own + i * p.classes)};
+        const uint32_t v = own + i * p.classes;
+        const uint4* const w[1] = {vectorsAt(v)};
         float z[T];
         dots<T>(w, h, ldh, p.dim, off, lane, z);
         const float x = warpSums(z, lane);
-        if (lane < T) run.take(x, c);
+        if constexpr (SLOPES) {
+            if (lane < T && row.live) giveSlope(p, t, v, row.take(p, x, p.first + v));
+        } else {
+            if (lane < T) run.take(x, c);
+        }
+    }
+    if constexpr (SLOPES) {
+        zeroSlopes(p, packed);
+        return;
     }
 #pragma unroll
     for (uint32_t o = T; o < T * kScoreAcross; o *= 2)
         fold(run.top, run.sum, __shfl_xor_sync(0xffffffffu, run.top, o), __shfl_xor_sync(0xffffffffu, run.sum, o), c);
-    if (lane < T) parts[warp][reversed<T>(lane)] = make_float2(run.top, run.sum);
+    if (lane < T) parts[warp][t] = make_float2(run.top, run.sum);
 
     // z where a list (a label) names an entry of this class, a warp an entry.
     for (uint32_t e = at; e < p.rows * p.entries; e += of) {
-        const uint32_t row = e / p.entries;
-        if (stateOf(p, row) != kLive) continue;
-        const uint32_t id = p.labels ? static_cast<uint32_t>(p.labels[row]) : p.ids[e];
+        const uint32_t to = e / p.entries;
+        if (stateOf(p, to) != kLive) continue;
+        const uint32_t id = p.labels ? static_cast<uint32_t>(p.labels[to]) : p.ids[e];
         if (id == kNoEntry || id % p.classes != own) continue;
         const uint4* const w[1] = {vectorsAt(id)};
         float z[1];
-        dots<1>(w, h + row * ldh, ldh, p.dim, off, lane, z);
+        dots<1>(w, h + to * ldh, ldh, p.dim, off, lane, z);
         const float x = warpSums(z, lane);
         if (lane == 0) p.listed[e] = x * p.scale;
     }
