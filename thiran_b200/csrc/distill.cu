@@ -19,6 +19,10 @@
 // Two CTAs share an SM, so that one's exponentials fill the other's folds and
 // waits. The folds have a fixed order: equal inputs give equal bits.
 //
+// Every wait is bounded. A warp whose wait ran out says so at the next barrier
+// of the CTA's computing warps, behind which none of them goes on: a row's list
+// names places in memory, and nobody uses one that was not handed over.
+//
 // When there are fewer rows than CTAs, a cluster of up to 8 shares a row and
 // its CTAs send each other their parts by asynchronous stores into
 // distributed shared memory.
@@ -31,6 +35,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -78,6 +83,7 @@ struct Params {
     const float* gradLoss;
     void* grad;
     uint32_t* status;
+    uint32_t spins;  // tries of a wait
 };
 
 // 16-byte vectors of logits as pairs of f32.
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
             uint32_t started = 0;  // bit per slot: a copy was started; its parity
             uint32_t parity = 0;
             for (uint64_t row = firstRow; row < p.rows && !abortFlag; row += step) {
-                if (!mbarWait(&listed[list], listPhase, &abortFlag)) { abortFlag = 1; break; }
+                if (!mbarWait(&listed[list], listPhase, &abortFlag, p.spins)) { abortFlag = 1; break; }
                 const int state = infos[list].state;
                 mbarArrive(&unlisted[list]);
                 if (++list == kLists) { list = 0; listPhase ^= 1u; }
@@ -278,7 +284,7 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
                 for (uint32_t i = 0; i < n + again; ++i) {
                     const uint32_t first = (i < n ? i : i - n) * kChunk;
                     const uint32_t bytes = min(seg.vectors - first, kChunk) * 16;
-                    if (!mbarWait(&empty[slot], phase ^ 1u, &abortFlag)) { abortFlag = 1; break; }
+                    if (!mbarWait(&empty[slot], phase ^ 1u, &abortFlag, p.spins)) { abortFlag = 1; break; }
                     mbarExpect(&full[slot], bytes);
                     bulkLoad(ring + slot * kChunk, data + first, bytes, &full[slot]);
                     started |= 1u << slot;
@@ -317,7 +323,7 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
         };
         readEarly(firstRow);
         for (uint64_t row = firstRow; row < p.rows; row += step) {
-            if (!mbarWait(&unlisted[at], phase ^ 1u, &abortFlag)) abortFlag = 1;
+            if (!mbarWait(&unlisted[at], phase ^ 1u, &abortFlag, p.spins)) abortFlag = 1;
             if (__any_sync(0xffffffffu, abortFlag)) break;
             const T* z = logitsOf(row);
             const Segment<T> seg(z, p.vocab, p.cluster, rank);
@@ -396,11 +402,25 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
         const float c = p.scale * kLog2e;
         const uint32_t fromLast = kConsumers - 1 - threadIdx.x;  // entries go to the last warps; the first one folds
         uint32_t slot = 0, phase = 0, at = 0, listPhase = 0, turn = 0, recPhase = 0;
-        auto consumerSync = [&] { asm volatile("barrier.sync 1, %0;" ::"n"(kConsumers) : "memory"); };
-        // A wait that runs out ends every later one at once; the rows still
-        // pass, with invalid results and the status word raised.
+        // A wait that runs out ends every later one at once.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            if (!mbarWait(bar, parity, &abortFlag)) abortFlag = 1;
+            if (mbarWait(bar, parity, &abortFlag, p.spins)) return true;
+            abortFlag = 1;
+            return false;
+        };
+        // A barrier of the computing warps: whether no wait has run out. A warp
+        // whose list did not come meets the others at their next barrier, and
+        // all leave behind it; those without another row meet it at one behind
+        // the loop.
+        auto agreed = [&] {
+            uint32_t all;
+            asm volatile(
+                "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, %2, p;\n"
+                " selp.u32 %0, 1, 0, q;\n}\n"
+                : "=r"(all)
+                : "r"(abortFlag ? 0u : 1u), "n"(kConsumers)
+                : "memory");
+            return all != 0;
         };
         auto advance = [&] {
             if (++slot == p.chunks) { slot = 0; phase ^= 1u; }
@@ -415,6 +435,7 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
         };
         const float2 none = make_float2(kLowest, 0.0f);
 
+        bool together = true;
         for (uint64_t row = firstRow; row < p.rows; row += step) {
             const Segment<T> seg(logitsOf(row), p.vocab, p.cluster, rank);
             T* grad = MODE == kScore ? nullptr : static_cast<T*>(p.grad) + row * p.ldGrad;
@@ -433,7 +454,10 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
                     }
                 }
             };
-            wait(&listed[at], listPhase);
+            if (!__all_sync(0xffffffffu, wait(&listed[at], listPhase))) {
+                together = agreed();
+                break;
+            }
             const RowInfo& info = infos[at];
             const int state = info.state;
             if (state != 1) {
@@ -493,7 +517,7 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
                     sum = warpSum((running.sum.x + running.sum.y + pow2((edge - running.top) * c)) *
                                   pow2((running.top - top) * c));
                     if (lane == 0) parts[turn][warp] = make_float2(top, sum);
-                    consumerSync();
+                    if (!(together = agreed())) break;
                     if (p.cluster == 1) {
                         sum = fold(lane < WARPS ? parts[turn][lane] : none, top);
                     } else {
@@ -557,7 +581,11 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
                         advance();
                     }
                     if (hasEdge) grad[seg.edge(threadIdx.x)] = Vec<T>::from(slope * probability(edge));
-                    consumerSync();
+                    if constexpr (MODE == kBackward) {
+                        if (!(together = agreed())) break;
+                    } else {
+                        asm volatile("barrier.sync 1, %0;" ::"n"(kConsumers) : "memory");  // all agreed on this row
+                    }
                     // The entries' places, behind the stores above: p less the
                     // shares of the id, which the first of equal ids writes.
                     const List list = listAt(at);
@@ -579,10 +607,16 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
             release(&unlisted[at]);
             if (++at == kLists) { at = 0; listPhase ^= 1u; }
         }
+        if (together) agreed();
     }
     __syncthreads();
     if (threadIdx.x == 0 && abortFlag) atomicOr(p.status, kWaitStatus);
-    if (p.cluster > 1) clusterSync();  // nothing is sent to a CTA that has left
+    if (p.cluster > 1) {
+        clusterSync();  // nothing is sent to a CTA that has left
+        // One that gave up has not counted what it was sent: those 16 bytes a
+        // CTA, under 2 us on their way, get 200.
+        for (uint32_t i = 0; abortFlag && i < 2000; ++i) __nanosleep(100);
+    }
 }
 
 cudaLaunchConfig_t configFor(uint32_t grid, uint32_t threads, uint32_t smemBytes, uint32_t cluster,
@@ -600,6 +634,16 @@ cudaLaunchConfig_t configFor(uint32_t grid, uint32_t threads, uint32_t smemBytes
     config.attrs = &attribute;
     config.numAttrs = 1;
     return config;
+}
+
+// Tries of a wait before it gives up (THB_WAIT_SPINS: fewer, to see what comes
+// of it).
+uint32_t waitSpins() {
+    static const uint32_t spins = [] {
+        const char* e = std::getenv("THB_WAIT_SPINS");
+        return e ? static_cast<uint32_t>(std::min<unsigned long long>(std::strtoull(e, nullptr, 10), kSpinLimit)) : kSpinLimit;
+    }();
+    return spins;
 }
 
 // Clusters of this shape that fit on the device at once.
@@ -664,6 +708,7 @@ cudaError_t launchTyped(const Problem& q, int smCount, uint32_t* status, cudaStr
     p.gradLoss = q.gradLoss;
     p.grad = q.gradLogits;
     p.status = status;
+    p.spins = waitSpins();
     p.chunks = chunks;
     const uint32_t smemBytes = p.chunks * kChunkBytes + lists;
     int device = 0;

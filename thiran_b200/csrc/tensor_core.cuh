@@ -14,7 +14,7 @@
 namespace thb::tc {
 
 constexpr uint32_t kWaitStatus = 16u;
-constexpr uint64_t kSpinLimit = 1ull << 24;
+constexpr uint32_t kSpinLimit = 1u << 24;
 
 __device__ __forceinline__ uint32_t smem(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -27,11 +27,12 @@ __device__ __forceinline__ void mbarExpect(uint64_t* b, uint32_t bytes) {
 __device__ __forceinline__ void mbarArrive(uint64_t* b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem(b)) : "memory");
 }
-// True when the phase with parity `parity` has completed; false on timeout,
-// or as soon as `abort` (when given) reads non-zero.
-__device__ __forceinline__ bool mbarWait(uint64_t* b, uint32_t parity, const volatile int* abort = nullptr) {
+// True when the phase with parity `parity` has completed; false after `limit`
+// tries (one at least), or as soon as `abort` (when given) reads non-zero.
+__device__ __forceinline__ bool mbarWait(uint64_t* b, uint32_t parity, const volatile int* abort = nullptr,
+                                         uint32_t limit = kSpinLimit) {
     const uint32_t addr = smem(b);
-    for (uint64_t spin = 0; spin < kSpinLimit; ++spin) {
+    for (uint32_t spin = 0;; ++spin) {
         uint32_t done;
         asm volatile(
             "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
@@ -39,9 +40,8 @@ __device__ __forceinline__ bool mbarWait(uint64_t* b, uint32_t parity, const vol
             : "r"(addr), "r"(parity)
             : "memory");
         if (done) return true;
-        if (abort && (spin & 255u) == 255u && *abort) return false;
+        if (spin + 1 >= limit || (abort && (spin & 255u) == 255u && *abort)) return false;
     }
-    return false;
 }
 
 // Whether the phase is complete, without a wait.
