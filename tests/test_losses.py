@@ -125,6 +125,37 @@ def test_more_refusals():
     refused("thb_distill_backward", distill_desc(grad_logits=None), says="grad_logits is null")
     refused("thb_distill_forward", distill_desc(loss=BIG), says="loss overlaps logits")
     refused(FORWARD, linear_desc(ld_weight=1 << 62), "GPU-SIZE-OVERFLOW")
+    far = 1 << 63  # of a single row, which steps nowhere
+    refused(BACKWARD, linear_desc(rows=1, ld_hidden=far, ld_grad_hidden=far, grad_hidden=BIG + 2), says="overlaps hidden")
+
+
+def side_by_side(columns, pitch):
+    """Slices of one buffer, `columns` bf16 apart, for hidden states and weights of width 32, and
+    f32 for logits of width 64."""
+    return (linear_desc(ld_hidden=pitch, ld_grad_hidden=pitch, grad_hidden=BIG + 2 * columns),
+            linear_desc(ld_weight=pitch, ld_grad_weight=pitch, grad_weight=2 * BIG + 2 * columns),
+            distill_desc(ld_logits=2 * pitch, ld_grad_logits=2 * pitch, grad_logits=BIG + 8 * columns))
+
+
+@pytest.mark.parametrize("columns,pitch", [(31, 64), (33, 64), (32, 63), (40, 71), (1, 64), (63, 64), (0, 64)])
+def test_slices_that_share_elements_are_refused(columns, pitch):
+    hidden, weight, logits = side_by_side(columns, pitch)
+    refused(BACKWARD, hidden, says="grad_hidden overlaps hidden")
+    refused(BACKWARD, weight, says="grad_weight overlaps weight")
+    if columns:  # (0: in place)
+        for name in ("thb_distill_forward", "thb_distill_backward"):
+            refused(name, logits, says="grad_logits overlaps logits")
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are nobody's")
+@pytest.mark.parametrize("columns,pitch", [(32, 64), (32, 65), (40, 72), (64 + 32, 64), (5 * 64 + 32, 64)])
+def test_slices_side_by_side_are_taken(columns, pitch):
+    """Arguments pass, and the device is what is missing."""
+    hidden, weight, logits = side_by_side(columns, pitch)
+    fail = C.create_string_buffer(1024)
+    for name, desc in ((BACKWARD, hidden), (BACKWARD, weight), ("thb_distill_forward", logits),
+                       ("thb_distill_backward", logits)):
+        assert getattr(thb.lib(), name)(0, C.byref(desc), None, fail, len(fail)) == thb.STATUS_BACKEND, fail.value
 
 
 def test_binding_refuses_wrong_tensors():

@@ -99,6 +99,7 @@ private:
 struct Extent {
     const char* name;
     std::uintptr_t begin = 0, end = 0;
+    std::uint64_t pitch = 0, width = 0;  // bytes from row to row, and of a row
 };
 
 // The bytes from the first to the last element of a [rows][ld] matrix.
@@ -115,11 +116,22 @@ Extent extentOf(const char* name, const void* p, std::uint64_t rows, std::uint64
         fail(Category::Validation, "GPU-SIZE-OVERFLOW", std::string(name) + ": size overflows");
     e.begin = reinterpret_cast<std::uintptr_t>(p);
     e.end = e.begin + size;
+    e.width = cols * bytes;
+    e.pitch = rows > 1 ? ld * bytes : e.width;
     return e;
 }
 
+// Whether two matrices share a byte. Column slices of one buffer, whose rows
+// take turns, do not; rows that step differently are taken as one piece.
+bool meet(const Extent& a, const Extent& b) {
+    if (a.begin >= b.end || b.begin >= a.end) return false;
+    if (a.pitch != b.pitch) return true;
+    if (a.begin > b.begin) return meet(b, a);
+    const std::uint64_t on = (b.begin - a.begin) % a.pitch;  // from a row of a to the next of b
+    return on < a.width || a.pitch - on < b.width;
+}
+
 void refuseOverlaps(const std::vector<Extent>& outputs, const std::vector<Extent>& inputs) {
-    auto meet = [](const Extent& a, const Extent& b) { return a.begin < b.end && b.begin < a.end; };
     for (std::size_t i = 0; i < outputs.size(); ++i) {
         for (std::size_t j = 0; j < i; ++j)
             if (meet(outputs[i], outputs[j])) badLoss(std::string(outputs[i].name) + " overlaps " + outputs[j].name);
