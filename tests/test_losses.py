@@ -1,6 +1,7 @@
 """The vocabulary losses without a device: the oracle's gradient against differences, and refusals."""
 import ctypes as C
 import os
+import re
 
 import pytest
 
@@ -201,3 +202,15 @@ def test_linear_losses_issue_tcgen05_and_tma():
         assert call in kernels and call in helpers
     for legacy in ("wgmma", "mma.sync", "wmma::"):
         assert legacy not in kernels + helpers
+
+
+def test_what_is_remembered_of_a_device_is_remembered_by_device():
+    """Function-local statics of the host code are tables by device, or hold nothing of a device."""
+    source = os.path.join(os.path.dirname(losses.__file__), "csrc")
+    for name in ("linear_loss.cu", "distill.cu"):
+        text = open(os.path.join(source, name)).read()
+        held = re.findall(r"^ +static (?!constexpr|__device__)(.*)$", text, re.M)
+        assert held
+        for line in held:
+            assert re.match(r"std::mutex mutex;|std::map<std::tuple<.*, int, .*known;|std::atomic<uint64_t> ready\{0\};|"
+                            r"std::atomic<uint32_t> pairs\[kKnownDevices\]\{\};|const uint32_t spins = ", line), (name, line)

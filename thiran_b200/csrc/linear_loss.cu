@@ -1377,10 +1377,19 @@ cudaError_t launch(void (*kernel)(Formal...), uint32_t grid, uint32_t block, uin
     return cudaLaunchKernelEx(&config, kernel, static_cast<Formal>(args)...);
 }
 
-// Clusters of two that fit on the device at once (SMs left over by the GPC
-// layout cannot host a pair).
+constexpr int kKnownDevices = 64;  // what is remembered of a device, is of the first 64
+
+// Clusters of two that fit on the current device at once (SMs left over by the
+// GPC layout, which differs from one GPU to the next, cannot host a pair);
+// asked once a device (`known`), a query that failed again with the next call.
 template <class Kernel>
-uint32_t residentPairs(Kernel kernel, uint32_t threads, uint32_t smemBytes, int smCount) {
+uint32_t residentPairs(Kernel kernel, uint32_t threads, uint32_t smemBytes, int smCount,
+                       std::atomic<uint32_t> (&known)[kKnownDevices]) {
+    const uint32_t fallback = static_cast<uint32_t>(smCount) / 2;
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return fallback;
+    if (device < kKnownDevices)
+        if (const uint32_t pairs = known[device].load(std::memory_order_relaxed)) return pairs;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(2);
     config.blockDim = dim3(threads);
@@ -1395,18 +1404,20 @@ uint32_t residentPairs(Kernel kernel, uint32_t threads, uint32_t smemBytes, int 
     int clusters = 0;
     if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) {
         (void)cudaGetLastError();
-        clusters = 0;
+        return fallback;
     }
-    return clusters > 0 ? static_cast<uint32_t>(clusters) : static_cast<uint32_t>(smCount) / 2;
+    if (clusters < 1) return fallback;
+    if (device < kKnownDevices) known[device].store(static_cast<uint32_t>(clusters), std::memory_order_relaxed);
+    return static_cast<uint32_t>(clusters);
 }
 
-// Lets the kernel use its shared memory, once a device (`ready`: the first 64).
+// Lets the kernel use its shared memory, once a device (`ready`).
 template <class Kernel>
 cudaError_t allowShared(Kernel kernel, uint32_t smemBytes, std::atomic<uint64_t>& ready) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
-    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    const uint64_t bit = device < kKnownDevices ? 1ull << device : 0;
     if (!bit || !(ready.load(std::memory_order_acquire) & bit)) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smemBytes));
         if (e != cudaSuccess) return e;
@@ -1425,7 +1436,8 @@ cudaError_t launchTyped(const CUtensorMap& a, const CUtensorMap& b, const Params
     if (e != cudaSuccess) return e;
     uint32_t slots = static_cast<uint32_t>(smCount);
     if constexpr (PAIR) {
-        static const uint32_t resident = residentPairs(kernel, threadsFor(EPI), smemBytes, smCount);
+        static std::atomic<uint32_t> pairs[kKnownDevices]{};
+        const uint32_t resident = residentPairs(kernel, threadsFor(EPI), smemBytes, smCount, pairs);
         slots = std::min(resident, static_cast<uint32_t>(smCount) / 2);
     }
     const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(maxTiles, slots)) * (PAIR ? 2u : 1u);
@@ -1484,7 +1496,8 @@ cudaError_t launchBoth(const CUtensorMap& slopesK, const CUtensorMap& weightMN, 
     if (e != cudaSuccess) return e;
     uint32_t units = static_cast<uint32_t>(smCount);
     if constexpr (PAIR) {
-        static const uint32_t resident = residentPairs(kernel, threadsFor(kEpiOut), smemBytes, smCount);
+        static std::atomic<uint32_t> pairs[kKnownDevices]{};
+        const uint32_t resident = residentPairs(kernel, threadsFor(kEpiOut), smemBytes, smCount, pairs);
         units = std::max(2u, std::min(resident, static_cast<uint32_t>(smCount) / 2));
     }
     if ((w.m + kBM - 1ull) / kBM * ((w.n + kBN - 1ull) / kBN) > UINT32_MAX / 2) return cudaErrorInvalidValue;
