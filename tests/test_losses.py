@@ -42,6 +42,27 @@ def test_oracle_agrees_with_torch():
     assert torch.allclose(ref.losses(z / 2, ref.teacher_lists(ids, s, 2.0))[0], divergence)
 
 
+def test_spreads_tell_how_sums_are_made():
+    """Sums of 1024 products keep the bound on lse; sums of the whole width and logits in bf16 do not.
+    Slopes of two summands keep the tighter bound on gradients, slopes of one only the wider."""
+    g = torch.Generator().manual_seed(3)
+    h, w, at = ref.well_known(24, 300, 4096, g, "cpu")
+    z = h.double() @ w.double().T
+    want = torch.logsumexp(z, 1)
+    assert ref.spread(torch.logsumexp(ref.cut_sums(h, w, 1024).double(), 1), want)[0] < ref.LSE_SPREAD
+    assert ref.spread(torch.logsumexp(ref.cut_sums(h, w, 4096).double(), 1), want)[0] > ref.LSE_SPREAD
+    assert ref.spread(torch.logsumexp(z.bfloat16().double(), 1), want)[0] > ref.LSE_SPREAD
+    h, w = torch.randn((48, 256), generator=g).bfloat16(), (torch.randn((500, 256), generator=g) / 8).bfloat16()
+    slope = ref.losses(h.double() @ w.double().T, ref.label_lists(torch.randint(0, 500, (48,), generator=g), 500))[2]
+    slope = slope * torch.rand((48, 1), generator=g)
+    first = slope.bfloat16().double()
+    second = first + (slope - first).bfloat16().double()
+    for rounded, tight in ((first, False), (second, True)):
+        for a, b, x in ((slope, rounded, w.double()), (slope.T, rounded.T, h.double())):
+            off = ref.spread((b @ x).bfloat16(), a @ x)[1]
+            assert off < ref.GRADIENT_SPREAD[tight] and (tight or off > ref.GRADIENT_SPREAD[True])
+
+
 def linear_desc(**changes):
     d = losses.LinearLossDesc(rows=16, vocab=64, dim=32, hidden=BIG, ld_hidden=32, weight=2 * BIG, ld_weight=32,
                               labels=3 * BIG, ignore_index=-100, entries=0, scale=1.0, loss=4 * BIG, lse=5 * BIG,
