@@ -484,7 +484,8 @@ int thb_device_check_status(int device, void* stream, char* failure, uint64_t fa
  * A row whose label is `ignore_index`, or whose list has no entry, has loss
  * and lse 0 and a gradient of zeros, and its hidden state or logits are not
  * used. The same id twice in a list counts twice. A label or id >= vocab (or
- * a negative label that is not ignore_index) makes that row's loss NaN,
+ * a negative label that is not ignore_index; an id even where its logit is
+ * -inf) makes that row's loss NaN,
  * leaves the row out of the gradients and latches TH-SPEC-BOUNDS in the
  * device status word (thb_device_check_status). Losses are per row; equal
  * inputs give equal bits.
@@ -497,14 +498,21 @@ int thb_device_check_status(int device, void* stream, char* failure, uint64_t fa
 /* z = scale * hidden weight^T, never stored: hidden bf16 [rows][ld_hidden],
  * weight bf16 [vocab][ld_weight] (leading dimensions in elements, any values
  * >= dim; weight rows that do not start at multiples of 16 bytes are copied
- * once per call, except for the forward pass of up to 8 rows). Exactly one of `labels` and the teacher's lists is given.
+ * once per call, except for the forward pass of up to 8 rows that fit shared
+ * memory, eight of a width of 6400). Exactly one of `labels` and the teacher's
+ * lists is given. Logits of any finite size are taken; lse and the slopes come
+ * from the same sums, so the backward call takes lse of a forward call with
+ * the same rows.
  * grad_loss f32 [rows] is each row's upstream gradient; grad_hidden and
  * grad_weight are bf16, whole tensors are written. Products accumulate in
  * f32; the slopes that enter the gradients' products are rounded to bf16 (of
  * up to 64 rows to the sum of two).
  * The workspace (256-byte aligned) carries nothing from call to call, but
  * belongs to one call at a time: streams or graphs that may run at the same
- * time need one each. Outputs overlap neither inputs nor each other. */
+ * time need one each. A call of fewer rows may need a larger one (its sums are
+ * split over more SMs), so that each size is to be asked for. Outputs share no
+ * element with inputs or each other (column slices of one buffer do not; of
+ * rows that step differently, the whole ranges are compared). */
 typedef struct thb_linear_loss_desc {
     uint64_t rows, vocab, dim;
     const void* hidden;

@@ -640,12 +640,14 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                         if (!live || j >= left) v[j] = 0.0f;
                 }
                 // The slopes are rounded to bf16, the tensor cores' operand
-                // type: as much as the gradients' own rounding. Where few rows
-                // leave the tile room, what the rounding left follows as rows
-                // of its own, whose products add to the same sums: the few
-                // slopes that such gradients consist of do not average their
-                // roundings out. (64 rows, 32768 x 2048: off by 0.0017 of the
-                // norm instead of 0.0024, 148 us a step instead of 140.)
+                // type: as much as the gradients' own rounding, so that a
+                // gradient is off by 0.0024 of its norm, of any number of
+                // rows, where f32 slopes leave 0.0017. Where the rows fill
+                // half a tile at most, what the rounding left follows as rows
+                // of its own in the other half, whose products add to the
+                // same sums: 0.0017 for little (64 rows, 32768 x 2048: 148 us
+                // a step instead of 140), while more rows would need as many
+                // tiles again.
                 __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.c);
                 if constexpr (!givesTwins(EPI)) {
                     storeSlopes(stage, c, p.ldc, row, 32u, col, v, lane);
@@ -1125,8 +1127,11 @@ __device__ __forceinline__ uint8_t rowState(const PlanParams& p, uint64_t row) {
 }
 
 // Packs the live rows. Each CTA takes a run of rows and counts the live ones
-// before it for itself: 8 bytes a row from L2, which for any number of rows
-// is small beside the row's dim * 2 bytes and needs no second launch.
+// before it for itself, which needs no second launch but reads every row's
+// label (8 bytes, or a state of 1) in every CTA, up to 4 an SM: 4.7 KB of L2
+// reads a row. At 8192 rows that is 39 MB, a few us; at a million rows of a
+// narrow head the largest part of the call (1048576 rows, 1000 x 64: 770 us of
+// 1900).
 __global__ void __launch_bounds__(kPlanThreads) planRows(const PlanParams p, uint32_t blocks, const Align align) {
     __shared__ uint32_t warpSums[2][kPlanThreads / 32];
     __shared__ uint32_t places[kPlanThreads];
@@ -1544,7 +1549,8 @@ constexpr uint64_t kMaxSplits = 128;
 // One after the other, dH takes at least the time to read the weights and dW
 // to write as much (6.5 and 3.7 TB/s); a tile of dW at least 1.6 to read out,
 // 4 where rows are no whole vectors. At the same time, on a part of the SMs
-// each, both take at least that of the mixed traffic (5 TB/s measured); few
+// each, both take at least that of the mixed traffic (4.5 to 5 TB/s is what
+// this kernel reaches, short of the 6.5 of a copy); few
 // SMs read less than they compute, 0.5 us a k block of a single CTA; and
 // products that fill the SMs lose about a tenth to shorter waves. So this wins
 // where launches and memory count (the gradients' call: 64 rows, 32768 x 2048

@@ -159,7 +159,8 @@ def _temperature(value):
 
 def linear_loss_workspace(rows, vocab, dim, entries=1, backward=True, aligned=None, device=0):
     """Bytes of workspace that a linear loss over these sizes needs. With `backward` it serves the
-    forward and the backward call. `entries` is the length of the teacher's lists (labels: 1);
+    forward and the backward call over these rows; fewer rows may need more, so each size is to be
+    asked for. `entries` is the length of the teacher's lists (labels: 1);
     `aligned` says whether every weight row starts at a multiple of 16 bytes (by default: whether
     contiguous rows do)."""
     if _lib is None:
@@ -215,8 +216,9 @@ def linear_cross_entropy(hidden, weight, labels, loss, lse, workspace, scale=1.0
 
 def linear_cross_entropy_backward(hidden, weight, labels, lse, grad_loss, grad_hidden, grad_weight, workspace,
                                   scale=1.0, ignore_index=-100, stream=0):
-    """Gradients of sum_t grad_loss[t] * loss[t] with respect to hidden and weight, from the
-    forward call's `lse`; z is computed again, a piece of the vocabulary at a time."""
+    """Gradients of sum_t grad_loss[t] * loss[t] with respect to hidden and weight, from the `lse` of
+    a forward call with the same rows; z is computed again, summed as it was there, a piece of the
+    vocabulary at a time."""
     desc, rows, vocab, dim, ordinal = _linear(hidden, weight, workspace, scale)
     desc.labels, desc.ignore_index = _vector("labels", labels, rows, _i64, ordinal), ignore_index
     _backward(desc, rows, vocab, dim, ordinal, lse, grad_loss, grad_hidden, grad_weight, stream)
