@@ -35,7 +35,6 @@
 
 #include <algorithm>
 #include <cstdint>
-#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -63,7 +62,6 @@ constexpr uint32_t kAhead = 2;   // chunks that a row never keeps from the copie
 constexpr uint32_t kLists = 3;   // rows whose lists are kept
 constexpr uint32_t kEdges = 16;
 constexpr uint32_t kNoEntry = 0x7fffffffu;
-constexpr uint32_t kDrainStatus = 32u;
 constexpr float kLowest = -3.402823466e38f;
 
 enum : int { kScore = 0, kTrain = 1, kBackward = 2 };
@@ -634,16 +632,6 @@ cudaLaunchConfig_t configFor(uint32_t grid, uint32_t threads, uint32_t smemBytes
     config.attrs = &attribute;
     config.numAttrs = 1;
     return config;
-}
-
-// Tries of a wait before it gives up (THB_WAIT_SPINS: fewer, to see what comes
-// of it).
-uint32_t waitSpins() {
-    static const uint32_t spins = [] {
-        const char* e = std::getenv("THB_WAIT_SPINS");
-        return e ? static_cast<uint32_t>(std::min<unsigned long long>(std::strtoull(e, nullptr, 10), kSpinLimit)) : kSpinLimit;
-    }();
-    return spins;
 }
 
 // Clusters of this shape that fit on the device at once.

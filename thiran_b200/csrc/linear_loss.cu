@@ -31,7 +31,8 @@
 // Past 128 rows CTA pairs (cta_group::2) work on tiles of 256 x up to 256, up
 // to there single CTAs on 128 x up to 256. Two more warps look up the targets
 // of the next tiles' rows. Every wait is bounded: on expiry the CTA raises bit 4 of
-// the status word, drains its copies and MMAs, frees TMEM and returns.
+// the status word, waits for its MMAs and for the copies in flight (a pair's
+// leader for those of both), frees TMEM and returns.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -172,6 +173,7 @@ struct Params {
     uint64_t splitStride;  // kEpiAcc: elements between the splits' C
     uint32_t accumulate;
     uint32_t* status;
+    uint32_t spins;  // tries of a wait
 };
 
 // An arrival that orders no memory: what it hands over are TMEM columns whose
@@ -179,6 +181,29 @@ struct Params {
 // global stores of the tile.
 __device__ __forceinline__ void mbarArriveClusterRelaxed(uint32_t clusterAddress) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(clusterAddress) : "memory");
+}
+
+__device__ __forceinline__ void storeCluster(uint32_t clusterAddress, uint32_t x) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(clusterAddress), "r"(x) : "memory");
+}
+
+// Whether the loads that were issued have landed, when a wait has run out. The
+// full barriers count those of `here` and of `peer` k blocks (a CTA alone: the
+// same), of which `bytes` each; this CTA has armed its own blocks' barriers for
+// both CTAs. A block that one of the two did not come to is armed for the other's
+// bytes, or counted down by its own missing ones. Blocks further back than the
+// ring were consumed.
+template <uint32_t STAGES>
+__device__ bool landed(uint64_t* full, uint32_t here, uint32_t peer, uint32_t bytes) {
+    const uint32_t end = max(here, peer);
+    bool all = true;
+    for (uint32_t i = end > STAGES ? end - STAGES : 0u; i < end; ++i) {
+        uint64_t* bar = &full[i % STAGES];
+        if (i >= here) mbarExpect(bar, bytes);
+        else if (i >= peer) mbarComplete(bar, bytes);
+        all &= mbarWait(bar, i / STAGES % 2u);
+    }
+    return all;
 }
 
 // Groups of p.group m blocks, walked down m within each n block.
@@ -304,6 +329,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
     __shared__ __align__(8) uint64_t full[G::stages], empty[G::stages], tmemFull[2], tmemEmpty[2], mmaDone;
     __shared__ __align__(8) uint64_t rowsFull[2], rowsEmpty[2];
     __shared__ uint32_t tmemSlot;
+    __shared__ uint32_t issuedHere, issuedByPeer;  // k blocks whose loads were issued; by the other CTA of a pair (leader)
     __shared__ volatile int abortFlag;
     __shared__ float2 parts[kLogitParts][32];  // of the rows' strips, and
     __shared__ bool lastOne;                 // whether this CTA joins them (finished)
@@ -368,9 +394,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
 
     if (warp == 0 && lane == 0) {
         // ---- TMA producer ----
-        uint32_t stage = 0, phase = 0;
-        uint32_t issuedParity[G::stages];
-        uint32_t issued = 0;
+        uint32_t stage = 0, phase = 0, issued = 0;
         for (uint32_t tile = first; tile < tiles && !abortFlag; tile += step) {
             uint32_t mb, nb;
             tileCoords(tile % plane, mTiles, p, mb, nb);
@@ -378,7 +402,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
             const int32_t row0 = static_cast<int32_t>(mb * G::tileM + rank * kBM);
             const int32_t col0 = static_cast<int32_t>(p.bFirstN + nb * tileN + rank * (tileN / 2));
             for (uint32_t kb = kb0; kb < kb1; ++kb) {
-                if (!mbarWait(&empty[stage], phase ^ 1u, &abortFlag)) { abortFlag = 1; break; }
+                if (!mbarWait(&empty[stage], phase ^ 1u, &abortFlag, p.spins)) { abortFlag = 1; break; }
                 uint8_t* a = base + stage * G::stageBytes;
                 uint8_t* b = a + kABytes;
                 const int32_t ka = static_cast<int32_t>(kb * kBK);
@@ -415,21 +439,15 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                         tmaLoad2d(b, &mapB, kB, col0, &full[stage]);
                     }
                 }
-                issuedParity[stage] = phase;
-                issued |= 1u << stage;
+                ++issued;
                 if (++stage == G::stages) { stage = 0; phase ^= 1u; }
             }
         }
-        if (abortFlag) {
-            // Loads already issued land before the CTA can exit. A pair counts
-            // them on the leader's barriers, which only the leader can wait
-            // on; the peer gives its loads a fixed 200 us instead.
-            if (!PAIR || rank == 0) {
-                for (int s = 0; s < G::stages; ++s)
-                    if (issued & (1u << s)) (void)mbarWait(&full[s], issuedParity[s]);
-            } else {
-                for (int i = 0; i < 2000; ++i) __nanosleep(100);
-            }
+        if constexpr (PAIR) {
+            if (rank == 0) issuedHere = issued;
+            else storeCluster(pairAddress(&issuedByPeer, 0), issued);
+        } else if (abortFlag && !landed<G::stages>(full, issued, issued, loadBytes)) {
+            atomicOr(p.status, kDrainStatus);
         }
     } else if (warp == 1 && lane == 0) {
         // ---- MMA issuer (of a pair: the leader, for both CTAs) ----
@@ -459,11 +477,11 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                 uint32_t kb = kb0;
                 do {  // one accumulator: the whole k range, or blocksPerSum of it
                     const uint32_t end = sumsLogits(EPI) ? min(kb + p.blocksPerSum, kb1) : kb1;
-                    if (!mbarWait(&tmemEmpty[acc], accPhase ^ 1u, &abortFlag)) { abortFlag = 1; ok = false; break; }
+                    if (!mbarWait(&tmemEmpty[acc], accPhase ^ 1u, &abortFlag, p.spins)) { abortFlag = 1; ok = false; break; }
                     fenceAfter();
                     const uint32_t d = tmemBase + acc * kBN;
                     for (const uint32_t begin = kb; kb < end; ++kb) {
-                        if (!ready && !mbarWait(&full[stage], phase, &abortFlag)) { abortFlag = 1; ok = false; break; }
+                        if (!ready && !mbarWait(&full[stage], phase, &abortFlag, p.spins)) { abortFlag = 1; ok = false; break; }
                         fenceAfter();
                         const uint32_t next = stage + 1 == G::stages ? 0u : stage + 1;
                         const uint32_t nextPhase = next ? phase : phase ^ 1u;
@@ -497,7 +515,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
             for (uint32_t tile = first; tile < tiles; tile += step) {
                 uint32_t mb, nb;
                 tileCoords(tile % plane, mTiles, p, mb, nb);
-                if (!mbarWait(&rowsEmpty[buf], phase ^ 1u, &abortFlag)) abortFlag = 1;
+                if (!mbarWait(&rowsEmpty[buf], phase ^ 1u, &abortFlag, p.spins)) abortFlag = 1;
                 if (__any_sync(0xffffffffu, abortFlag)) break;
                 TileRows& out = tileRows[buf];
                 constexpr uint32_t kRows = kBM / (32 * kListWarps);  // of a thread
@@ -589,7 +607,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
             float rowScale = 0.0f, minusLse = 0.0f;
             uint64_t outRow = row;
             if constexpr (usesLists(EPI)) {
-                if (!mbarWait(&rowsFull[rowsBuf], rowsPhase, &abortFlag)) abortFlag = 1;
+                if (!mbarWait(&rowsFull[rowsBuf], rowsPhase, &abortFlag, p.spins)) abortFlag = 1;
                 if (__any_sync(0xffffffffu, abortFlag)) break;  // the warp leaves together
                 const TileRows& in = tileRows[rowsBuf];
                 const uint32_t r = quadrant * 32 + lane;
@@ -672,7 +690,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                 uint32_t raw[kStrip / 32][32];
                 auto z = [&](uint32_t j) { return __uint_as_float(raw[j / 32][j % 32]); };
                 auto arrived = [&] {  // (The warp leaves together.)
-                    if (!mbarWait(&tmemFull[acc], accPhase, &abortFlag)) abortFlag = 1;
+                    if (!mbarWait(&tmemFull[acc], accPhase, &abortFlag, p.spins)) abortFlag = 1;
                     if (__any_sync(0xffffffffu, abortFlag)) return false;
                     fenceAfter();
                     return true;
@@ -744,7 +762,7 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                 }
                 continue;
             }
-            if (!mbarWait(&tmemFull[acc], accPhase, &abortFlag)) abortFlag = 1;
+            if (!mbarWait(&tmemFull[acc], accPhase, &abortFlag, p.spins)) abortFlag = 1;
             if (__any_sync(0xffffffffu, abortFlag)) break;
             fenceAfter();
             // 32 columns at a time, the next ones on their way meanwhile.
@@ -855,8 +873,15 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
         }
     }
     // A pair stays resident until both CTAs are done: the leader's MMAs read
-    // the peer's shared memory and the peer arrives on the leader's barriers.
-    if constexpr (PAIR) clusterSync();
+    // the peer's shared memory, the peer arrives on the leader's barriers, and
+    // loads in flight, which both CTAs count there, land before either leaves.
+    if constexpr (PAIR) {
+        clusterSync();
+        if (rank == 0 && threadIdx.x == 0 && (abortFlag || issuedHere != issuedByPeer) &&
+            !landed<G::stages>(full, issuedHere, issuedByPeer, loadBytes))
+            atomicOr(p.status, kWaitStatus | kDrainStatus);
+        clusterSync();
+    }
     if (warp == 1) {
         fenceAfter();
         if constexpr (PAIR)
@@ -1831,6 +1856,7 @@ cudaError_t forward(const Problem& q, int smCount, std::uint32_t* status, cudaSt
     p.strips = place<float2>(q, l.strips);
     p.stripLd = l.rowsPad;
     p.status = status;
+    p.spins = waitSpins();
     // Rows that the last CTA of the products joins by itself, saving a launch
     // where a call is little more than its launches. (128 rows would take it
     // 37 us instead of the 5 of joinStrips.)
@@ -1877,6 +1903,7 @@ cudaError_t backward(const Problem& q, int smCount, std::uint32_t* status, cudaS
     base.count = place<uint32_t>(q, l.count);
     base.splits = 1;
     base.status = status;
+    base.spins = waitSpins();
     for (uint64_t i = 0; i < l.pieces; ++i) {
         const uint64_t first = i * l.piece, width = std::min(l.piece, q.vocab - first);
         Params s = base;

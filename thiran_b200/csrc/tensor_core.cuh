@@ -8,12 +8,15 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <cstdlib>
 #include <mutex>
 
 namespace thb::tc {
 
-constexpr uint32_t kWaitStatus = 16u;
+constexpr uint32_t kWaitStatus = 16u;   // a bounded wait ran out
+constexpr uint32_t kDrainStatus = 32u;  // so did the one for copies in flight
 constexpr uint32_t kSpinLimit = 1u << 24;
 
 __device__ __forceinline__ uint32_t smem(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -26,6 +29,10 @@ __device__ __forceinline__ void mbarExpect(uint64_t* b, uint32_t bytes) {
 }
 __device__ __forceinline__ void mbarArrive(uint64_t* b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem(b)) : "memory");
+}
+// Counts `bytes` on a barrier in place of a copy that does not come.
+__device__ __forceinline__ void mbarComplete(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem(b)), "r"(bytes) : "memory");
 }
 // True when the phase with parity `parity` has completed; false after `limit`
 // tries (one at least), or as soon as `abort` (when given) reads non-zero.
@@ -189,6 +196,16 @@ __device__ __forceinline__ void tmemArrived(uint32_t (&r)[32]) {
 }
 
 // ---- host ----
+
+// Tries of a wait before it gives up (THB_WAIT_SPINS: fewer, to see what comes
+// of it).
+inline uint32_t waitSpins() {
+    static const uint32_t spins = [] {
+        const char* e = std::getenv("THB_WAIT_SPINS");
+        return e ? static_cast<uint32_t>(std::min<unsigned long long>(std::strtoull(e, nullptr, 10), kSpinLimit)) : kSpinLimit;
+    }();
+    return spins;
+}
 
 inline PFN_cuTensorMapEncodeTiled_v12000 encodeFn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
