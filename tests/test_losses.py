@@ -147,8 +147,6 @@ def test_more_refusals():
     refused("thb_distill_backward", distill_desc(grad_logits=None), says="grad_logits is null")
     refused("thb_distill_forward", distill_desc(loss=BIG), says="loss overlaps logits")
     refused(FORWARD, linear_desc(ld_weight=1 << 62), "GPU-SIZE-OVERFLOW")
-    far = 1 << 63  # of a single row, which steps nowhere
-    refused(BACKWARD, linear_desc(rows=1, ld_hidden=far, ld_grad_hidden=far, grad_hidden=BIG + 2), says="overlaps hidden")
 
 
 def side_by_side(columns, pitch):
@@ -167,6 +165,11 @@ def test_slices_that_share_elements_are_refused(columns, pitch):
     if columns:  # (0: in place)
         for name in ("thb_distill_forward", "thb_distill_backward"):
             refused(name, logits, says="grad_logits overlaps logits")
+
+
+def test_a_single_row_steps_nowhere():
+    far = 1 << 63
+    refused(BACKWARD, linear_desc(rows=1, ld_hidden=far, ld_grad_hidden=far, grad_hidden=BIG + 2), says="overlaps hidden")
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are nobody's")
