@@ -17,7 +17,7 @@ namespace thb::tc {
 
 constexpr uint32_t kWaitStatus = 16u;   // a bounded wait ran out
 constexpr uint32_t kDrainStatus = 32u;  // so did the one for copies in flight
-constexpr uint32_t kSpinLimit = 1u << 24;
+constexpr uint64_t kSpinLimit = 1ull << 24;
 
 __device__ __forceinline__ uint32_t smem(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -34,20 +34,32 @@ __device__ __forceinline__ void mbarArrive(uint64_t* b) {
 __device__ __forceinline__ void mbarComplete(uint64_t* b, uint32_t bytes) {
     asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem(b)), "r"(bytes) : "memory");
 }
-// True when the phase with parity `parity` has completed; false after `limit`
-// tries (one at least), or as soon as `abort` (when given) reads non-zero.
-__device__ __forceinline__ bool mbarWait(uint64_t* b, uint32_t parity, const volatile int* abort = nullptr,
-                                         uint32_t limit = kSpinLimit) {
+// Waits a while, as the hardware sees fit, for the phase with parity `parity`.
+__device__ __forceinline__ uint32_t mbarTry(uint32_t addr, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    return done;
+}
+// True when the phase with parity `parity` has completed; false on timeout,
+// or as soon as `abort` (when given) reads non-zero.
+__device__ __forceinline__ bool mbarWait(uint64_t* b, uint32_t parity, const volatile int* abort = nullptr) {
+    const uint32_t addr = smem(b);
+    for (uint64_t spin = 0; spin < kSpinLimit; ++spin) {
+        if (mbarTry(addr, parity)) return true;
+        if (abort && (spin & 255u) == 255u && *abort) return false;
+    }
+    return false;
+}
+// The same with a limit of its own: `limit` tries, one at least.
+__device__ __forceinline__ bool mbarWait(uint64_t* b, uint32_t parity, const volatile int* abort, uint32_t limit) {
     const uint32_t addr = smem(b);
     for (uint32_t spin = 0;; ++spin) {
-        uint32_t done;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-            : "=r"(done)
-            : "r"(addr), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if (spin + 1 >= limit || (abort && (spin & 255u) == 255u && *abort)) return false;
+        if (mbarTry(addr, parity)) return true;
+        if (spin + 1 >= limit || ((spin & 255u) == 255u && *abort)) return false;
     }
 }
 
