@@ -238,3 +238,16 @@ def test_what_is_remembered_of_a_device_is_remembered_by_device():
         for line in held:
             assert re.match(r"std::mutex mutex;|std::map<std::tuple<.*, int, .*known;|std::atomic<uint64_t> ready\{0\};|"
                             r"std::atomic<uint32_t> pairs\[kKnownDevices\]\{\};|const uint32_t spins = ", line), (name, line)
+
+
+def test_copies_in_flight_are_waited_for_behind_the_last_role():
+    """Any role's wait may run out after the copies' own role has left, so their wait stands behind
+    the barrier at which all roles have ended."""
+    source = os.path.join(os.path.dirname(losses.__file__), "csrc")
+    for name, end, drains in (("distill.cu", "\n    __syncthreads();\n    if (threadIdx.x == 0 && abortFlag)", ["drained &= mbarWait("]),
+                              ("linear_loss.cu", "\n    __syncthreads();\n    if (threadIdx.x == 0 && abortFlag)",
+                               ["!landed<G::stages>(full, issuedHere, issuedByPeer", "!landed<G::stages>(full, issuedHere, issuedHere"])):
+        text = open(os.path.join(source, name)).read()
+        assert text.count(end) == 1
+        for drain in drains:
+            assert text.count(drain) == 1 and text.index(drain) > text.index(end), (name, drain)

@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
     __shared__ float2 parts[2][WARPS];
     __shared__ RowInfo infos[kLists];
     __shared__ volatile int abortFlag;
+    __shared__ uint32_t started, parity;  // bit per slot: a copy was started; its parity
 
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = p.cluster > 1 ? blockIdx.x % p.cluster : 0u;
@@ -268,8 +269,7 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
         // ---- copies ----
         if (lane == 0) {
             uint32_t slot = 0, phase = 0, list = 0, listPhase = 0;
-            uint32_t started = 0;  // bit per slot: a copy was started; its parity
-            uint32_t parity = 0;
+            uint32_t begun = 0, phases = 0;  // started, parity
             for (uint64_t row = firstRow; row < p.rows && !abortFlag; row += step) {
                 if (!mbarWait(&listed[list], listPhase, &abortFlag, p.spins)) { abortFlag = 1; break; }
                 const int state = infos[list].state;
@@ -285,17 +285,13 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
                     if (!mbarWait(&empty[slot], phase ^ 1u, &abortFlag, p.spins)) { abortFlag = 1; break; }
                     mbarExpect(&full[slot], bytes);
                     bulkLoad(ring + slot * kChunk, data + first, bytes, &full[slot]);
-                    started |= 1u << slot;
-                    parity = (parity & ~(1u << slot)) | phase << slot;
+                    begun |= 1u << slot;
+                    phases = (phases & ~(1u << slot)) | phase << slot;
                     if (++slot == p.chunks) { slot = 0; phase ^= 1u; }
                 }
             }
-            if (abortFlag) {
-                bool drained = true;  // copies in flight land before the CTA exits
-                for (uint32_t i = 0; i < p.chunks; ++i)
-                    if (started >> i & 1u) drained &= mbarWait(&full[i], parity >> i & 1u);
-                atomicOr(p.status, kWaitStatus | (drained ? 0u : kDrainStatus));
-            }
+            started = begun;
+            parity = phases;
         }
     } else if (warp == WARPS + 1) {
         // ---- lists ----
@@ -608,7 +604,13 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
         if (together) agreed();
     }
     __syncthreads();
-    if (threadIdx.x == 0 && abortFlag) atomicOr(p.status, kWaitStatus);
+    if (threadIdx.x == 0 && abortFlag) {
+        // Whoever gave up: copies in flight land before the CTA leaves.
+        bool drained = true;
+        for (uint32_t i = 0; i < p.chunks; ++i)
+            if (started >> i & 1u) drained &= mbarWait(&full[i], parity >> i & 1u);
+        atomicOr(p.status, kWaitStatus | (drained ? 0u : kDrainStatus));
+    }
     if (p.cluster > 1) {
         clusterSync();  // nothing is sent to a CTA that has left
         // One that gave up has not counted what it was sent: those 16 bytes a

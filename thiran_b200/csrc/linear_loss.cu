@@ -187,8 +187,8 @@ __device__ __forceinline__ void storeCluster(uint32_t clusterAddress, uint32_t x
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(clusterAddress), "r"(x) : "memory");
 }
 
-// Whether the loads that were issued have landed, when a wait has run out. The
-// full barriers count those of `here` and of `peer` k blocks (a CTA alone: the
+// Whether the loads that were issued have landed, when a wait has run out,
+// whoever's (all roles have ended). The full barriers count those of `here` and of `peer` k blocks (a CTA alone: the
 // same), of which `bytes` each; this CTA has armed its own blocks' barriers for
 // both CTAs. A block that one of the two did not come to is armed for the other's
 // bytes, or counted down by its own missing ones. Blocks further back than the
@@ -443,12 +443,8 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
                 if (++stage == G::stages) { stage = 0; phase ^= 1u; }
             }
         }
-        if constexpr (PAIR) {
-            if (rank == 0) issuedHere = issued;
-            else storeCluster(pairAddress(&issuedByPeer, 0), issued);
-        } else if (abortFlag && !landed<G::stages>(full, issued, issued, loadBytes)) {
-            atomicOr(p.status, kDrainStatus);
-        }
+        if (rank == 0) issuedHere = issued;
+        else storeCluster(pairAddress(&issuedByPeer, 0), issued);
     } else if (warp == 1 && lane == 0) {
         // ---- MMA issuer (of a pair: the leader, for both CTAs) ----
         if (!PAIR || rank == 0) {
@@ -881,6 +877,8 @@ __device__ __forceinline__ void products(const CUtensorMap& mapA, const CUtensor
             !landed<G::stages>(full, issuedHere, issuedByPeer, loadBytes))
             atomicOr(p.status, kWaitStatus | kDrainStatus);
         clusterSync();
+    } else if (threadIdx.x == 0 && abortFlag && !landed<G::stages>(full, issuedHere, issuedHere, loadBytes)) {
+        atomicOr(p.status, kDrainStatus);
     }
     if (warp == 1) {
         fenceAfter();
