@@ -251,3 +251,10 @@ def test_copies_in_flight_are_waited_for_behind_the_last_role():
         assert text.count(end) == 1
         for drain in drains:
             assert text.count(drain) == 1 and text.index(drain) > text.index(end), (name, drain)
+
+
+def test_no_wait_is_a_mere_sleep():
+    """What is in flight is counted, not given a while."""
+    source = os.path.join(os.path.dirname(losses.__file__), "csrc")
+    for name in ("linear_loss.cu", "linear_score.cuh", "distill.cu"):
+        assert "nanosleep" not in open(os.path.join(source, name)).read()

@@ -209,6 +209,31 @@ __device__ __forceinline__ void bulkLoad(void* dst, const void* src, uint32_t by
                  : "memory");
 }
 
+// Whether all that the cluster's CTAs have sent here has landed. Row j is
+// counted on barrier j % 2, which this CTA arms when it sends its own part;
+// rows before its last were waited for, and no CTA is more than one ahead. After
+// an expired wait, parts that were not sent are counted in their place, and
+// those of a row that this CTA did not come to are armed.
+__device__ bool partsLanded(uint64_t* received, uint32_t here, const uint32_t* by, uint32_t cluster, bool gaveUp) {
+    uint32_t missing = 0, ahead = 0;
+    for (uint32_t k = 0; k < cluster; ++k) {
+        missing += by[k] < here;
+        ahead += by[k] > here;
+    }
+    if (!gaveUp && !missing && !ahead) return true;
+    bool all = true;
+    if (here) {
+        const uint32_t last = here - 1;
+        if (missing) mbarComplete(&received[last % 2], 16 * missing);
+        all = mbarWait(&received[last % 2], last / 2 % 2);
+    }
+    if (ahead) {
+        mbarExpect(&received[here % 2], 16 * ahead);
+        all &= mbarWait(&received[here % 2], here / 2 % 2);
+    }
+    return all;
+}
+
 // A row as the list warp hands it over.
 struct RowInfo {
     int state;        // 0: no target, 1: live, 2: an id outside the vocabulary
@@ -230,6 +255,7 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
     __shared__ RowInfo infos[kLists];
     __shared__ volatile int abortFlag;
     __shared__ uint32_t started, parity;  // bit per slot: a copy was started; its parity
+    __shared__ uint32_t sentHere, sentBy[kMaxCluster];  // rows whose part this CTA, each CTA has sent the cluster
 
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = p.cluster > 1 ? blockIdx.x % p.cluster : 0u;
@@ -251,6 +277,7 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
 
     if (threadIdx.x == 0) {
         abortFlag = 0;
+        sentHere = 0;
         for (uint32_t i = 0; i < kMaxChunks; ++i) {
             mbarInit(&full[i], 1);
             mbarInit(&empty[i], WARPS);
@@ -517,7 +544,10 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
                     } else {
                         if (warp == 0) {
                             sum = fold(lane < WARPS ? parts[turn][lane] : none, top);
-                            if (lane == 0) mbarExpect(&received[turn], 16 * p.cluster);
+                            if (lane == 0) {
+                                mbarExpect(&received[turn], 16 * p.cluster);
+                                ++sentHere;
+                            }
                             if (lane < p.cluster)
                                 sendTo(lane, &records[turn][rank], &received[turn], make_float4(top, sum, 0.0f, 0.0f));
                         }
@@ -612,10 +642,10 @@ __global__ void __launch_bounds__(32 * WARPS + 64, WARPS >= 8 ? 2 : 6) distillRo
         atomicOr(p.status, kWaitStatus | (drained ? 0u : kDrainStatus));
     }
     if (p.cluster > 1) {
+        if (threadIdx.x < p.cluster) storeCluster(pairAddress(&sentBy[rank], threadIdx.x), sentHere);
         clusterSync();  // nothing is sent to a CTA that has left
-        // One that gave up has not counted what it was sent: those 16 bytes a
-        // CTA, under 2 us on their way, get 200.
-        for (uint32_t i = 0; abortFlag && i < 2000; ++i) __nanosleep(100);
+        if (threadIdx.x == 0 && !partsLanded(received, sentHere, sentBy, p.cluster, abortFlag))
+            atomicOr(p.status, kWaitStatus | kDrainStatus);
     }
 }
 

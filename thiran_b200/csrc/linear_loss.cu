@@ -183,10 +183,6 @@ __device__ __forceinline__ void mbarArriveClusterRelaxed(uint32_t clusterAddress
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(clusterAddress) : "memory");
 }
 
-__device__ __forceinline__ void storeCluster(uint32_t clusterAddress, uint32_t x) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(clusterAddress), "r"(x) : "memory");
-}
-
 // Whether the loads that were issued have landed, when a wait has run out,
 // whoever's (all roles have ended). The full barriers count those of `here` and of `peer` k blocks (a CTA alone: the
 // same), of which `bytes` each; this CTA has armed its own blocks' barriers for

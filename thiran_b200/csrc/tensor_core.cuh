@@ -120,6 +120,10 @@ __device__ __forceinline__ uint32_t pairAddress(const void* p, uint32_t rank) {
     return a;
 }
 
+__device__ __forceinline__ void storeCluster(uint32_t clusterAddress, uint32_t x) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(clusterAddress), "r"(x) : "memory");
+}
+
 // All threads of both CTAs.
 __device__ __forceinline__ void clusterSync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
